@@ -13,6 +13,7 @@ from __future__ import annotations
 import glob
 import hashlib
 import os
+import subprocess
 import threading
 
 import torch
@@ -69,6 +70,16 @@ def is_current() -> bool:
         return f.read().strip() == _source_hash()
 
 
+def _cxx_runtime() -> list[str]:
+    """Link flag for the shared C++ runtime where the toolchain offers only the static one by default.
+    A second, static copy of it beside torch's crashes as soon as a check's message prints a number."""
+    try:
+        found = subprocess.run(["g++", "-print-file-name=libstdc++.so.6"], capture_output=True, text=True).stdout.strip()
+    except OSError:
+        return []
+    return ["-l:libstdc++.so.6"] if os.path.isabs(found) else []
+
+
 def build(verbose: bool = False) -> str:
     """Compile every CUDA source for sm_100a into ``_build/r9k_C.so`` (cross-compiles without a GPU)."""
     from torch.utils.cpp_extension import load
@@ -83,6 +94,7 @@ def build(verbose: bool = False) -> str:
         extra_cflags=CXX_FLAGS,
         extra_cuda_cflags=NVCC_FLAGS,
         extra_include_paths=[CSRC_DIR],
+        extra_ldflags=_cxx_runtime(),
         build_directory=BUILD_DIR,
         verbose=verbose,
         is_python_module=False,
