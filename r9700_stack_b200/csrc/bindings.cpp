@@ -147,6 +147,15 @@ void sparse_mla_decode_tc(torch::Tensor q, torch::Tensor lat_cache, torch::Tenso
                           torch::Tensor sel, torch::Tensor sel_count, double scale, torch::Tensor part_o,
                           torch::Tensor part_ml, torch::Tensor out, torch::Tensor status);
 void head_gemv(torch::Tensor x, torch::Tensor W, torch::Tensor out);
+void plan_step(torch::Tensor new_len, torch::Tensor state, torch::Tensor block_table, torch::Tensor ring, int64_t cap,
+               int64_t window, int64_t sinks, torch::Tensor out);
+void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,
+                      torch::Tensor seq_start, torch::Tensor seq_len, torch::Tensor tok_ctx, double sm_scale,
+                      double k_scale, double v_scale, int64_t window, int64_t sinks, c10::optional<torch::Tensor> gate,
+                      torch::Tensor out, int64_t max_new, int64_t max_ctx, torch::Tensor status);
+void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperature, c10::optional<torch::Tensor> top_k,
+                   c10::optional<torch::Tensor> top_p, c10::optional<torch::Tensor> min_p, torch::Tensor tokens,
+                   torch::Tensor logprobs);
 void host_gather(torch::Tensor table, torch::Tensor ids, int64_t fmt, int64_t dim, torch::Tensor out);
 void moe_gather_bf16(torch::Tensor x, int64_t k, torch::Tensor perm_row, torch::Tensor out);
 void ngram_ids(torch::Tensor ids, torch::Tensor seq_start, torch::Tensor seq_len, torch::Tensor seq_slot,
@@ -323,6 +332,13 @@ TORCH_LIBRARY(r9k, m) {
   m.def("gdn_decode_fused(Tensor proj, int Hk, int Hv, int z_off, int b_off, int a_off, Tensor conv_w, "
         "Tensor(a!) conv_state, Tensor(b!) state, Tensor seq_slot, Tensor seq_has_state, Tensor A_log, "
         "Tensor dt_bias, Tensor norm_w, float eps, Tensor(c!)? out_q, Tensor(d!)? out_sf, Tensor(e!)? out_bf16) -> ()");
+  m.def("plan_step(Tensor new_len, Tensor state, Tensor(a!) block_table, Tensor(b!) ring, int cap, int window, "
+        "int sinks, Tensor(c!) out) -> ()");
+  m.def("window_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_start, "
+        "Tensor seq_len, Tensor tok_ctx, float sm_scale, float k_scale, float v_scale, int window, int sinks, "
+        "Tensor? gate, Tensor(a!) out, int max_new, int max_ctx, Tensor(b!) status) -> ()");
+  m.def("sample_logits(Tensor logits, Tensor u, Tensor temperature, Tensor? top_k, Tensor? top_p, Tensor? min_p, "
+        "Tensor(a!) tokens, Tensor(b!) logprobs) -> ()");
   m.def("gdn_out_norm_quant(Tensor o, Tensor proj, int z_off, Tensor w, float eps, Tensor(a!)? y, "
         "Tensor(b!)? out_q, Tensor(c!)? out_sf) -> ()");
 }
@@ -391,6 +407,9 @@ TORCH_LIBRARY_IMPL(r9k, CUDA, m) {
   m.impl("lru_route", &r9k::lru_route);
   m.impl("expert_copy", &r9k::expert_copy);
   m.impl("gdn_recurrent", &r9k::gdn_recurrent);
+  m.impl("plan_step", &r9k::plan_step);
+  m.impl("window_attention", &r9k::window_attention);
+  m.impl("sample_logits", &r9k::sample_logits);
   m.impl("gdn_out_norm_quant", &r9k::gdn_out_norm_quant);
   m.impl("gdn_decode_fused", &r9k::gdn_decode_fused);
   m.impl("gdn_state_prefetch", &r9k::gdn_state_prefetch);
