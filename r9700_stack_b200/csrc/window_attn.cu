@@ -3,9 +3,14 @@
 // A query at position p (its context is p + 1) sees key j iff j <= p and (W = 0 or j > p - W or
 // j < S): the last W positions, its own among them, and the first S tokens of the sequence.
 //   o = softmax(q K^T * scale) V, then o * sigmoid(gate) where a gate is given, rounded to bf16 once.
-// Queries keep their bf16 value and probabilities about that of bf16 (the kernels of attention_tc.cu
-// round both to one e4m3 number). A row that sees no key is zero. Keys outside the visible range are
-// never used, whatever their pages hold.
+// A row that sees no key is zero. Keys outside the visible range are never used, whatever their pages
+// hold.
+//
+// Precision. The cache stays e4m3 in shared memory, where the MMA reads it; the other operand of each
+// product is the sum of two e4m3 numbers, both multiplied into the same fp32 accumulator: a query q as
+// hi + lo after a power-of-two scaling of its row (exact for |q| >= amax / 1792, else within
+// 2^-19 amax), a probability p as hi + lo (within 2^-8 of itself, or 2^-16 of the row's largest). Two
+// e4m3 products cost what one bf16 product does, and no key or value has to be widened on the way.
 //
 // KV cache layout: [pages][kv_heads][64][head_dim] e4m3 for K and V separately.
 #include <torch/extension.h>
@@ -13,11 +18,13 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <climits>
 #include "common.cuh"
+#include "tmap.h"
 
 namespace r9k {
 
 namespace wa {
 constexpr int PAGE = 64;
+constexpr int KT = 128;  // keys of a tile: the MMA's M (single tokens) or N (chunks)
 
 struct Args {
   const __nv_bfloat16* q;  // [T, Hq, D], token stride ld_q
@@ -32,73 +39,1003 @@ struct Args {
   __nv_bfloat16* out;         // [T, Hq * D], token stride ld_out
   int64_t ld_gate, ld_out;
   int T, S, Hq, Hkv, G, width, pages, window, sinks, max_new;
-  float scale;    // sm_scale * k_scale
+  float scale_log2;  // sm_scale * k_scale, for powers of two
   float v_scale;
   int* status;
+  uint64_t timeout_ns;
 };
+
+// The visible keys of a group of rows as tiles of KT keys: first the sinks [0, sk), then the window
+// [base, lim) from a page boundary on.
+struct Span {
+  int base, lim, sk, n_sink, n;
+  R9K_DEVINL int key0(int j) const { return j < n_sink ? j * KT : base + (j - n_sink) * KT; }
+  R9K_DEVINL int end(int j) const { return j < n_sink ? sk : lim; }
+};
+
+// ctx_min, ctx_max: smallest and largest context of the rows that see anything (0, 0: none does)
+R9K_DEVINL Span make_span(const Args& a, int ctx_min, int ctx_max) {
+  Span s;
+  const int lo = a.window > 0 ? max(0, ctx_min - a.window) : 0;
+  s.base = lo / PAGE * PAGE;
+  s.lim = ctx_max;
+  s.sk = min(a.sinks, s.base);
+  s.n_sink = (s.sk + KT - 1) / KT;
+  s.n = s.n_sink + (ctx_max > s.base ? (ctx_max - s.base + KT - 1) / KT : 0);
+  return s;
+}
+
+R9K_DEVINL bool visible(const Args& a, int key, int ctx) {
+  return key < ctx && (a.window == 0 || key >= ctx - a.window || key < a.sinks);
+}
+
+// a token's context, cut to what its table row can hold
+R9K_DEVINL int context(const Args& a, int tok) {
+  const int c = a.tok_ctx[tok];
+  if (c > a.width * PAGE) {
+    report_error(a.status, kErrBounds, 301, c);
+    return a.width * PAGE;
+  }
+  return max(c, 0);
+}
+
+// smallest (of the positive ones) and largest context of n tokens from tok0 on; one warp
+R9K_DEVINL void context_range(const Args& a, int tok0, int n, int& lo, int& hi) {
+  lo = INT_MAX;
+  hi = 0;
+  for (int i = lane_id(); i < n; i += 32) {
+    const int c = context(a, tok0 + i);
+    if (c > 0) lo = min(lo, c);
+    hi = max(hi, c);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if (hi == 0) lo = 0;
+}
+
+R9K_DEVINL int page_of(const Args& a, int seq, int key) {
+  const int p = a.table[(int64_t)seq * a.width + key / PAGE];
+  if ((unsigned)p >= (unsigned)a.pages) {
+    report_error(a.status, kErrBounds, 302, p);
+    return 0;
+  }
+  return p;
+}
+
+// K or V tile j -> shared memory: two pages, D / 128 column halves, 128-byte swizzled rows. A page past
+// the tile's end is not looked up (its rows are masked): page 0 stands in for it.
+template <int D>
+R9K_DEVINL void load_tile(const Args& a, const CUtensorMap* map, uint8_t* dst, uint64_t* bar, const Span& sp, int j, int seq,
+                          int kvh) {
+  const int key0 = sp.key0(j), end = sp.end(j);
+  mbar_arrive_expect_tx(bar, KT * D);
+#pragma unroll
+  for (int p = 0; p < KT / PAGE; ++p) {
+    const int key = key0 + p * PAGE;
+    const int page = key < end ? page_of(a, seq, key) : 0;
+#pragma unroll
+    for (int h = 0; h < D / 128; ++h)
+      tma_load_2d(dst + h * (KT * 128) + p * (PAGE * 128), map, bar, h * 128, (page * a.Hkv + kvh) * PAGE);
+  }
+}
+
+// operand descriptor, MN-major 128-byte swizzle (values: head dims contiguous, keys along K)
+R9K_DEVINL uint64_t sdesc_mn(uint32_t saddr) {
+  uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)((KT * 128) >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+
+R9K_DEVINL float ld_dsmem(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+R9K_DEVINL uint32_t e4m3x2(float lo, float hi) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+R9K_DEVINL float2 f32x2(uint32_t e) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)e, __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+// (hi, lo) e4m3 pairs of two numbers: x ~ hi + lo
+R9K_DEVINL void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = e4m3x2(x, y);
+  const float2 b = f32x2(hi);
+  lo = e4m3x2(x - b.x, y - b.y);
+}
+
+// 16 bf16 of a row -> 16 bytes hi and lo, scaled
+R9K_DEVINL void split16(const uint4 (&r)[2], float inv, uint4& hi, uint4& lo) {
+  const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(r);
+  uint32_t* ph = reinterpret_cast<uint32_t*>(&hi);
+  uint32_t* pl = reinterpret_cast<uint32_t*>(&lo);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h0, l0, h1, l1;
+    split2(__bfloat162float(e[4 * i]) * inv, __bfloat162float(e[4 * i + 1]) * inv, h0, l0);
+    split2(__bfloat162float(e[4 * i + 2]) * inv, __bfloat162float(e[4 * i + 3]) * inv, h1, l1);
+    ph[i] = h0 | (h1 << 16);
+    pl[i] = l0 | (l1 << 16);
+  }
+}
+R9K_DEVINL float amax16(const uint4 (&r)[2]) {
+  const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(r);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(__bfloat162float(e[i])));
+  return m;
+}
+
+// Probabilities are exp2(s - m_ref + P_SHIFT): m_ref follows the running maximum once that has grown by
+// P_LAG (O is rescaled then), so the largest lies in [2^6.5, 2^8.75], below e4m3's 448, and the lo
+// part's 2^-10 is 2^-16.5 of it or less.
+constexpr float P_SHIFT = 6.5f, P_LAG = 2.25f;
+
+// One value row (key r of a tile, every column half) whose key some of the rows do not see. A NaN code
+// in it would reach those rows too (0 * NaN), so such a row of values is cleared, and the rows that do
+// see its key are marked: they become NaN as a whole. Values of keys that no row sees are stale bytes.
+template <int D>
+R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, int end, int tok0, int ntok, int* poison) {
+  uint32_t nan = 0;
+#pragma unroll
+  for (int h = 0; h < D / 128; ++h)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + h * (KT * 128) + r * 128 + ((c ^ (r & 7)) << 4));
+      nan |= ((v.x & 0x7f7f7f7fu) + 0x01010101u) | ((v.y & 0x7f7f7f7fu) + 0x01010101u) |
+             ((v.z & 0x7f7f7f7fu) + 0x01010101u) | ((v.w & 0x7f7f7f7fu) + 0x01010101u);
+    }
+  if ((nan & 0x80808080u) == 0) return;
+  for (int i = 0; i < ntok; ++i)
+    if (key < end && visible(a, key, context(a, tok0 + i))) poison[i] = 1;
+#pragma unroll
+  for (int h = 0; h < D / 128; ++h)
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      *reinterpret_cast<uint4*>(tile + h * (KT * 128) + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+}
 }  // namespace wa
 
-// One warp a (token, query head) row; a lane holds D / 32 of its dims; running maximum and sum.
+// ------------------------------------------------------------------------------------------------
+// Single tokens and a few drafts: up to 16 rows (tokens x heads of one kv head's group) of a sequence.
+//
+// The 128 keys of a tile are the MMA's M rows and the query rows its N = 16 columns, so no product is
+// spent on padding rows: S^T = K Q^T [keys x rows], O^T += V^T P^T [dims x rows], both in TMEM. K and V
+// tiles share one ring of shared-memory slots in the order in which the MMAs use them (K0 K1 V0 K2 V1
+// ...). Warp 0 loads (TMA), warp 1 issues MMAs, warps 2-5 hold one key a thread: they mask, find the
+// column maxima together, and write the probabilities as two e4m3 planes.
+// The CTAs of a cluster take neighbouring shares of the tiles; at the end each of them sums a share of
+// the dims over the others' partial results in distributed shared memory, and writes the output.
+// ------------------------------------------------------------------------------------------------
+namespace wd {
+using namespace wa;
+constexpr int N = 16;          // query rows of a tile
+constexpr int THREADS = 192;
 template <int D>
-__global__ void __launch_bounds__(128) window_attn_simple_kernel(const wa::Args a) {
-  using namespace wa;
+struct Cfg {
+  static constexpr int HALVES = D / 128;
+  static constexpr int UNIT = KT * D;                 // one K or V tile
+  static constexpr int SLOTS = D == 256 ? 3 : 6;      // two CTAs on an SM
+  static constexpr int PLANE_Q = HALVES * N * 128;    // hi or lo plane of Q: a swizzled tile a half
+  static constexpr int PLANE_P = N * 128;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_RING = OFF_Q + 2 * PLANE_Q;
+  static constexpr int OFF_P = OFF_RING + SLOTS * UNIT;  // [parity][hi, lo]
+  static constexpr int OFF_RED = OFF_P + 4 * PLANE_P;    // float [parity][max, sum][4 warps][N]
+  static constexpr int OFF_COL = OFF_RED + 2 * 2 * 4 * N * 4;  // scale[N], ctx[N], poison[N], m[N], l[N]
+  static constexpr int OFF_BAR = OFF_COL + 5 * N * 4;
+  static constexpr int NBAR = 1 + 2 * SLOTS + 8;  // q_full, full[], empty[], s_full[2], s_free[2], p_full[2], pv_done[2]
+  static constexpr int OFF_TMEM = OFF_BAR + NBAR * 8;
+  static constexpr int SMEM = OFF_TMEM + 16 + 1024;
+};
+constexpr int TMEM_COLS = 64;
+constexpr int S_COL = 0, O_COL = 32;  // S buffers [0, 32), O^T halves [32, 64)
+}  // namespace wd
+
+R9K_DEVINL void wd_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+template <int D, int NC>
+__global__ void __launch_bounds__(wd::THREADS, 2)
+    window_attn_dec_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const wa::Args a) {
+  using namespace wd;
+  using C = Cfg<D>;
   pdl_wait();
   pdl_trigger();
-  constexpr int PER = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int h = blockIdx.y * 4 + (threadIdx.x >> 5);
-  const int seq = blockIdx.z, j = blockIdx.x;
-  if (h >= a.Hq) return;
-  const int t0 = a.seq_start[seq], len = a.seq_len[seq];
-  if (len > a.max_new && j == 0 && h == 0 && lane == 0) report_error(a.status, kErrConfig, 300, len);
-  if (j >= len) return;
-  if (t0 < 0 || t0 + len > a.T) {
-    if (lane == 0) report_error(a.status, kErrBounds, 300, t0);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bars;
+  uint64_t* full = bars + 1;
+  uint64_t* empty = full + C::SLOTS;
+  uint64_t* s_full = empty + C::SLOTS;
+  uint64_t* s_free = s_full + 2;
+  uint64_t* p_full = s_free + 2;
+  uint64_t* pv_done = p_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEM);
+  float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
+  float* col_scale = reinterpret_cast<float*>(smem + C::OFF_COL);
+  int* col_ctx = reinterpret_cast<int*>(col_scale + N);
+  int* poison = col_ctx + N;  // by token
+  float* col_m = reinterpret_cast<float*>(poison + N);
+  float* col_l = col_m + N;
+  __shared__ int s_fail;
+
+  const int warp = warp_id(), lane = lane_id();
+  const int seq = blockIdx.x, kvh = blockIdx.y;
+  const int nsplit = gridDim.z, split = blockIdx.z;
+  const int tok0 = a.seq_start[seq], ntok = a.seq_len[seq];
+  // the same decision in every CTA of the cluster: nobody is left at its barrier
+  if (ntok <= 0) return;
+  if (ntok > a.max_new || tok0 < 0 || tok0 > a.T - ntok) {
+    if (threadIdx.x == 0) report_error(a.status, ntok > a.max_new ? kErrConfig : kErrBounds, 310, ntok);
     return;
   }
-  const int t = t0 + j;
-  int ctx = a.tok_ctx[t];
-  if (ctx > a.width * PAGE) {
-    if (lane == 0) report_error(a.status, kErrBounds, 301, ctx);
-    ctx = a.width * PAGE;
-  }
-  const int lo = a.window > 0 ? max(0, ctx - a.window) : 0;
-  const int ns = min(a.sinks, lo);
-  float qv[PER], acc[PER], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    qv[i] = __bfloat162float(a.q[(int64_t)t * a.ld_q + h * D + lane + 32 * i]) * a.scale;
-    acc[i] = 0.f;
-  }
-  const int kvh = h / a.G;
-  for (int i = 0; i < ns + ctx - lo; ++i) {
-    const int key = i < ns ? i : lo + i - ns;
-    const int page = a.table[(int64_t)seq * a.width + key / PAGE];
-    if ((unsigned)page >= (unsigned)a.pages) {
-      if (lane == 0) report_error(a.status, kErrBounds, 302, page);
-      continue;
+  int ctx_min, ctx_max;
+  context_range(a, tok0, ntok, ctx_min, ctx_max);
+  const Span sp = make_span(a, ctx_min, ctx_max);
+  const int share = (sp.n + nsplit - 1) / nsplit;
+  const int j0 = min(sp.n, split * share), n = min(sp.n, j0 + share) - j0;
+  const int NQ = ntok * a.G;  // <= NC
+
+  if (threadIdx.x == 0) {
+    s_fail = 0;
+    mbar_init(q_full, 128);
+    for (int s = 0; s < C::SLOTS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
     }
-    const int64_t base = (((int64_t)page * a.Hkv + kvh) * PAGE + key % PAGE) * D + lane;
-    float s = 0.f;
-#pragma unroll
-    for (int c = 0; c < PER; ++c) s += qv[c] * e4m3_to_f32(a.k[base + 32 * c]);
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float mn = fmaxf(m, s);
-    if (mn == -INFINITY) continue;  // no weight yet, and none in this key
-    const float corr = __expf(m - mn), pw = __expf(s - mn);
-    l = l * corr + pw;
-#pragma unroll
-    for (int c = 0; c < PER; ++c) acc[c] = acc[c] * corr + pw * e4m3_to_f32(a.v[base + 32 * c]);
-    m = mn;
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_free[s], 128);
+      mbar_init(&p_full[s], 128);
+      mbar_init(&pv_done[s], 1);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
   }
-  const float inv = l > 0.f || l != l ? a.v_scale / l : 0.f;
-#pragma unroll
-  for (int c = 0; c < PER; ++c) {
-    const int d = h * D + lane + 32 * c;
-    float o = acc[c] * inv;
-    if (a.gate != nullptr) o *= sigmoid_f(__bfloat162float(a.gate[(int64_t)t * a.ld_gate + d]));
-    a.out[(int64_t)t * a.ld_out + d] = __float2bfloat16(o);
+  if (threadIdx.x < N) poison[threadIdx.x] = 0;
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, TMEM_COLS);
+    tmem_relinquish();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_holder;
+  // the order of use: K0, then K(j + 1) (if there is one) and V(j)
+  auto unit_v = [&](int j) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int u = 0; u < 2 * n; ++u) {
+        const bool is_k = u == 0 || ((u & 1) && u < 2 * n - 1);
+        const int j = is_k ? (u + 1) / 2 : (u == 2 * n - 1 ? n - 1 : u / 2 - 1);
+        const int s = u % C::SLOTS;
+        if (!mbar_wait(&empty[s], (uint32_t)(((u / C::SLOTS) & 1) ^ 1), a.timeout_ns)) {
+          report_error(a.status, kErrMbarTimeout, 311, u);
+          break;
+        }
+        load_tile<D>(a, is_k ? &tmK : &tmV, smem + C::OFF_RING + s * C::UNIT, &full[s], sp, j0 + j, seq, kvh);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t idesc_s = idesc_dense(kFmtE4M3, kFmtE4M3, KT, N);
+      constexpr uint32_t idesc_o = idesc_dense(kFmtE4M3, kFmtE4M3, 128, N) | (1u << 15);  // A (V^T) MN-major
+      const uint32_t sq = smem_u32(smem + C::OFF_Q);
+      bool ok = mbar_wait(q_full, 0, a.timeout_ns);
+      auto slot = [&](int u) -> uint32_t { return smem_u32(smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT); };
+      auto wait_unit = [&](int u) { return mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns); };
+      auto issue_s = [&](int j) -> bool {
+        const int s = j & 1, u = j == 0 ? 0 : 2 * j - 1;
+        if (!wait_unit(u)) return false;
+        if (!mbar_wait(&s_free[s], (uint32_t)(((j >> 1) & 1) ^ 1), a.timeout_ns)) return false;
+        tc_fence_after();
+        const uint32_t sk = slot(u);
+#pragma unroll
+        for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int pl = 0; pl < 2; ++pl)
+              mma_f8f6f4_ss(tbase + S_COL + s * N, sdesc_k_sw128(sk + h * (KT * 128) + 32 * k),
+                            sdesc_k_sw128(sq + pl * C::PLANE_Q + h * (N * 128) + 32 * k), idesc_s,
+                            (h > 0 || k > 0 || pl > 0) ? 1u : 0u);
+        tc_commit(&s_full[s]);
+        tc_commit(&empty[u % C::SLOTS]);
+        return true;
+      };
+      if (ok) ok = issue_s(0);
+      for (int j = 0; ok && j < n; ++j) {
+        if (j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
+        const int pb = j & 1, u = unit_v(j);
+        if (!mbar_wait(&p_full[pb], (uint32_t)((j >> 1) & 1), a.timeout_ns)) { ok = false; break; }
+        if (!wait_unit(u)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t sv = slot(u), spp = smem_u32(smem + C::OFF_P + pb * 2 * C::PLANE_P);
+#pragma unroll
+        for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int pl = 0; pl < 2; ++pl)
+              mma_f8f6f4_ss(tbase + O_COL + h * N, sdesc_mn(sv + h * (KT * 128) + k * 4096),
+                            sdesc_k_sw128(spp + pl * C::PLANE_P + 32 * k), idesc_o, (j > 0 || k > 0 || pl > 0) ? 1u : 0u);
+        tc_commit(&pv_done[pb]);
+        tc_commit(&empty[u % C::SLOTS]);
+      }
+      if (!ok) report_error(a.status, kErrMbarTimeout, 312, 0);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    const int r = q * 32 + lane;      // TMEM lane: key of the tile, then dim of the output
+    const int tr = threadIdx.x - 64;  // 0..127
+    // rows of P past NQ stay zero; eight threads a query row
+    for (int i = tr; i < 4 * C::PLANE_P / 16; i += 128) reinterpret_cast<uint4*>(smem + C::OFF_P)[i] = make_uint4(0, 0, 0, 0);
+    {
+      const int row = tr >> 3, part = tr & 7;
+      const bool valid = row < NQ;
+      const int tok = tok0 + row / a.G, head = kvh * a.G + row % a.G;
+      constexpr int CH = D / 128;  // 16-element chunks a thread
+      uint4 raw[CH][2];
+      float amax = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int e0 = (c * 8 + part) * 16;
+        if (valid) {
+          const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + head * D + e0);
+          raw[c][0] = src[0];
+          raw[c][1] = src[1];
+        } else {
+          raw[c][0] = raw[c][1] = make_uint4(0, 0, 0, 0);
+        }
+        amax = fmaxf(amax, amax16(raw[c]));
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const int e = mx_exponent(amax, 448.f);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        uint4 hi, lo;
+        split16(raw[c], exp2i(-e), hi, lo);
+        uint8_t* dst = smem + C::OFF_Q + c * (N * 128) + row * 128 + ((part ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = hi;
+        *reinterpret_cast<uint4*>(dst + C::PLANE_Q) = lo;
+      }
+      if (part == 0) {
+        col_scale[row] = a.scale_log2 * exp2i(max(e, -126));
+        col_ctx[row] = valid ? context(a, tok) : 0;
+      }
+      fence_proxy_async();
+      mbar_arrive(q_full);
+    }
+    wd_bar();
+    float mref[NC], lsum[NC], csc[NC];
+    int cctx[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      mref[c] = -INFINITY;
+      lsum[c] = 0.f;
+      csc[c] = col_scale[c];
+      cctx[c] = col_ctx[c];
+    }
+    // a wait that runs out only raises s_fail: the loop is left at the end of a tile, by all together
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int s = j & 1, pb = j & 1;
+      bool w_ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns));
+      tc_fence_after();
+      float sv[16];
+      tmem_ld16(tbase + ((uint32_t)(q * 32) << 16) + S_COL + s * N, sv);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(&s_free[s]);
+      const int key0 = sp.key0(j0 + j), end = sp.end(j0 + j);
+      const int key = key0 + r;
+      // every row sees the whole tile: no key of it has to be masked
+      const bool whole = key0 + KT <= min(ctx_min, end) && (a.window == 0 || key0 >= ctx_max - a.window);
+      float* rmax = red + pb * 8 * N;
+      float* rsum = rmax + 4 * N;
+      float mx[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const bool vis = key < end && visible(a, key, cctx[c]);
+        sv[c] = vis ? sv[c] * csc[c] : -INFINITY;
+        mx[c] = sv[c];
+      }
+      if (!whole) {
+        const int u = unit_v(j);
+        w_ok &= __all_sync(0xffffffffu, mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns));
+        clean_value_row<D>(a, smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT, r, key, end, tok0, ntok, poison);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], o));
+      if (lane == 0) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) rmax[q * N + c] = mx[c];
+      }
+      wd_bar();
+      float fac[16];
+      bool any = false;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) fac[c] = 1.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float t = fmaxf(fmaxf(rmax[c], rmax[N + c]), fmaxf(rmax[2 * N + c], rmax[3 * N + c]));
+        const bool first = mref[c] == -INFINITY;
+        if (!first && t > mref[c] + P_LAG) {
+          fac[c] = exp2f(mref[c] - t);
+          any = true;
+          mref[c] = t;
+        } else if (first) {
+          mref[c] = t;
+        }
+      }
+      // P buffer pb is free once the PV of tile j - 2 is done; O is complete before it is rescaled
+      if (j >= 2) w_ok &= __all_sync(0xffffffffu, mbar_wait(&pv_done[pb], (uint32_t)(((j - 2) >> 1) & 1), a.timeout_ns));
+      if (any && j >= 1) {
+        w_ok &= __all_sync(0xffffffffu, mbar_wait(&pv_done[(j - 1) & 1], (uint32_t)(((j - 1) >> 1) & 1), a.timeout_ns));
+        tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < C::HALVES; ++h) {
+          const uint32_t orow = tbase + ((uint32_t)(q * 32) << 16) + O_COL + h * N;
+          float o[16];
+          tmem_ld16(orow, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] *= fac[i];
+          tmem_st16(orow, o);
+        }
+        tmem_st_wait();
+      }
+      uint8_t* prow = smem + C::OFF_P + pb * 2 * C::PLANE_P;
+      float ps[NC];
+#pragma unroll
+      for (int c = 0; c < NC; c += 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ps[c + i] = sv[c + i] == -INFINITY ? 0.f : exp2f(sv[c + i] - mref[c + i] + P_SHIFT);
+        uint32_t hi, lo;
+        split2(ps[c], ps[c + 1], hi, lo);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint8_t* dst = prow + (c + i) * 128 + ((((r >> 4) ^ ((c + i) & 7)) << 4) | (r & 15));
+          dst[0] = (uint8_t)(hi >> (8 * i));
+          dst[C::PLANE_P] = (uint8_t)(lo >> (8 * i));
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) ps[c] += __shfl_xor_sync(0xffffffffu, ps[c], o);
+      if (lane == 0) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) rsum[q * N + c] = ps[c];
+      }
+      if (!w_ok && lane == 0) atomicOr(&s_fail, 1);
+      fence_proxy_async();
+      tc_fence_before();
+      mbar_arrive(&p_full[pb]);
+      wd_bar();
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        lsum[c] = lsum[c] * fac[c] + ((rsum[c] + rsum[N + c]) + (rsum[2 * N + c] + rsum[3 * N + c]));
+      if (s_fail) {
+        ok = false;
+        break;
+      }
+    }
+    if (ok && n > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(n - 1) & 1], (uint32_t)(((n - 1) >> 1) & 1), a.timeout_ns));
+      tc_fence_after();
+    }
+    if (!ok) report_error(a.status, kErrMbarTimeout, 313, r);
+    // this CTA's partial results [row][dim], over the ring (all its tiles have been used)
+    if (n > 0 && ok) {
+      float* part = reinterpret_cast<float*>(smem + C::OFF_RING);
+#pragma unroll
+      for (int h = 0; h < C::HALVES; ++h) {
+        float o[16];
+        tmem_ld16(tbase + ((uint32_t)(q * 32) << 16) + O_COL + h * N, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < NC; ++c) part[c * D + h * 128 + r] = o[c];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (tr == c) {
+        col_m[c] = n > 0 && ok ? mref[c] : -INFINITY;
+        col_l[c] = n > 0 && ok ? lsum[c] : 0.f;
+      }
+    wd_bar();
+    if (tr < NQ && poison[tr / a.G]) col_l[tr] = __int_as_float(0x7fffffff);
+  }
+  tc_fence_before();
+  if (nsplit > 1) cluster_sync();
+  else __syncthreads();
+
+  // each CTA of the cluster joins a share of the dims of every row
+  {
+    const int dn = D / nsplit;
+    const uint32_t part = smem_u32(smem + C::OFF_RING), ml = smem_u32(col_m);
+    for (int i = threadIdx.x; i < NQ * dn; i += THREADS) {
+      const int row = i / dn, d = split * dn + i % dn;
+      float M = -INFINITY, L = 0.f, acc = 0.f;
+      for (int s = 0; s < nsplit; ++s) {
+        const uint32_t b = nsplit > 1 ? mapa_shared(ml, (uint32_t)s) : ml;
+        const float l = ld_dsmem(b + (N + row) * 4);
+        if (l != 0.f) M = fmaxf(M, ld_dsmem(b + row * 4));
+      }
+      for (int s = 0; s < nsplit; ++s) {
+        const uint32_t b = nsplit > 1 ? mapa_shared(ml, (uint32_t)s) : ml;
+        const uint32_t p = nsplit > 1 ? mapa_shared(part, (uint32_t)s) : part;
+        const float l = ld_dsmem(b + (N + row) * 4);
+        if (l == 0.f) continue;
+        const float m = ld_dsmem(b + row * 4);
+        const float w = m == -INFINITY ? 1.f : exp2f(m - M);
+        L += w * l;
+        acc += w * ld_dsmem(p + (row * D + d) * 4);
+      }
+      float o = L != 0.f ? acc / L * a.v_scale : 0.f;
+      const int tok = tok0 + row / a.G, col = (kvh * a.G + row % a.G) * D + d;
+      if (a.gate != nullptr) o *= sigmoid_f(__bfloat162float(a.gate[(int64_t)tok * a.ld_gate + col]));
+      a.out[(int64_t)tok * a.ld_out + col] = __float2bfloat16(o);
+    }
+  }
+  if (nsplit > 1) cluster_sync();  // peers read this CTA's shared memory until here
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Chunks: a tile of up to 128 rows (128 / G tokens x the G heads of one kv head's group), rows on the
+// MMA's M side.
+//
+// S = Q K^T [rows x keys] with two S buffers in TMEM, so the next tile's product runs during this
+// tile's softmax; O += P V with V read as it lies (MN-major B operand), O in TMEM. One thread a row
+// reads its scores, keeps the running maximum and sum and writes the probabilities (hi and lo plane).
+// K and V tiles share a ring of slots in the order of use, as above. Few tiles: a cluster of CTAs
+// shares the keys of a tile and joins the partial results through distributed shared memory.
+// ------------------------------------------------------------------------------------------------
+namespace wc {
+using namespace wa;
+constexpr int ROWS = 128;
+constexpr int THREADS = 192;
+template <int D>
+struct Cfg {
+  static constexpr int HALVES = D / 128;
+  static constexpr int UNIT = KT * D;
+  static constexpr int SLOTS = 4;
+  static constexpr int PLANE_Q = ROWS * D;
+  static constexpr int PLANE_P = ROWS * KT;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_RING = OFF_Q + 2 * PLANE_Q;
+  static constexpr int OFF_P = OFF_RING + SLOTS * UNIT;
+  static constexpr int OFF_ML = OFF_P + 2 * PLANE_P;    // m[ROWS], l[ROWS]
+  static constexpr int OFF_POISON = OFF_ML + 2 * ROWS * 4;  // by token
+  static constexpr int OFF_BAR = OFF_POISON + ROWS * 4;
+  static constexpr int NBAR = 1 + 2 * SLOTS + 6;  // q_full, full[], empty[], s_full[2], s_free[2], p_full, pv_done
+  static constexpr int OFF_TMEM = OFF_BAR + NBAR * 8;
+  static constexpr int SMEM = OFF_TMEM + 16 + 1024;
+  static constexpr int TMEM_COLS = 512;
+  static_assert(SMEM <= 232448, "shared memory");
+  static_assert(SLOTS * UNIT >= ROWS * D * 4, "the ring holds the partial results");
+};
+constexpr int O_COL = 0, S_COL = 256;
+}  // namespace wc
+
+template <int D>
+__global__ void __launch_bounds__(wc::THREADS, 1)
+    window_attn_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const wa::Args a) {
+  using namespace wc;
+  using C = Cfg<D>;
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bars;
+  uint64_t* full = bars + 1;
+  uint64_t* empty = full + C::SLOTS;
+  uint64_t* s_full = empty + C::SLOTS;
+  uint64_t* s_free = s_full + 2;
+  uint64_t* p_full = s_free + 2;
+  uint64_t* pv_done = p_full + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEM);
+  float* row_m = reinterpret_cast<float*>(smem + C::OFF_ML);
+  float* row_l = row_m + ROWS;
+  int* poison = reinterpret_cast<int*>(smem + C::OFF_POISON);
+
+  const int warp = warp_id(), lane = lane_id();
+  const int kvh = blockIdx.y;
+  const int nsplit = gridDim.z, split = blockIdx.z;
+  const int per = ROWS / a.G;  // tokens of a tile
+
+  // the sequence and the tokens of this tile: tiles are numbered through the sequences
+  int seq = -1, tok0 = 0, ntok = 0;
+  {
+    int before = 0;
+    for (int s0 = 0; s0 < a.S && seq < 0; s0 += 32) {
+      const int len = s0 + lane < a.S ? max(a.seq_len[s0 + lane], 0) : 0;
+      const int tiles = len > a.max_new ? 0 : (len + per - 1) / per;
+      int inc = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (blockIdx.x == 0 && blockIdx.y == 0 && split == 0 && warp == 0 && len > a.max_new)
+        report_error(a.status, kErrConfig, 320, len);
+      const uint32_t hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + inc);
+      if (hit != 0) {
+        const int src = __ffs((int)hit) - 1;
+        const int first = (int)blockIdx.x - before - (__shfl_sync(0xffffffffu, inc - tiles, src));
+        seq = s0 + src;
+        tok0 = first * per;
+        ntok = min(per, __shfl_sync(0xffffffffu, len, src) - tok0);
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  if (seq < 0) return;  // the grid is a bound: the same in the whole cluster
+  {
+    const int start = a.seq_start[seq], len = a.seq_len[seq];
+    if (start < 0 || start > a.T - len) {
+      if (threadIdx.x == 0) report_error(a.status, kErrBounds, 321, start);
+      return;
+    }
+    tok0 += start;
+  }
+  int ctx_min, ctx_max;
+  context_range(a, tok0, ntok, ctx_min, ctx_max);
+  const Span sp = make_span(a, ctx_min, ctx_max);
+  const int share = (sp.n + nsplit - 1) / nsplit;
+  const int j0 = min(sp.n, split * share), n = min(sp.n, j0 + share) - j0;
+  const int nrows = ntok * a.G;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 128);
+    for (int s = 0; s < C::SLOTS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&s_free[s], 128);
+    }
+    mbar_init(p_full, 128);
+    mbar_init(pv_done, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  if (threadIdx.x < ROWS) poison[threadIdx.x] = 0;
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_holder;
+  auto unit_v = [&](int j) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int u = 0; u < 2 * n; ++u) {
+        const bool is_k = u == 0 || ((u & 1) && u < 2 * n - 1);
+        const int j = is_k ? (u + 1) / 2 : (u == 2 * n - 1 ? n - 1 : u / 2 - 1);
+        const int s = u % C::SLOTS;
+        if (!mbar_wait(&empty[s], (uint32_t)(((u / C::SLOTS) & 1) ^ 1), a.timeout_ns)) {
+          report_error(a.status, kErrMbarTimeout, 322, u);
+          break;
+        }
+        load_tile<D>(a, is_k ? &tmK : &tmV, smem + C::OFF_RING + s * C::UNIT, &full[s], sp, j0 + j, seq, kvh);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t idesc_s = idesc_dense(kFmtE4M3, kFmtE4M3, ROWS, KT);
+      constexpr uint32_t idesc_o = idesc_dense(kFmtE4M3, kFmtE4M3, ROWS, D) | (1u << 16);  // B (V) MN-major
+      const uint32_t sq = smem_u32(smem + C::OFF_Q), spp = smem_u32(smem + C::OFF_P);
+      bool ok = mbar_wait(q_full, 0, a.timeout_ns);
+      auto slot = [&](int u) -> uint32_t { return smem_u32(smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT); };
+      auto wait_unit = [&](int u) { return mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns); };
+      auto issue_s = [&](int j) -> bool {
+        const int s = j & 1, u = j == 0 ? 0 : 2 * j - 1;
+        if (!wait_unit(u)) return false;
+        if (!mbar_wait(&s_free[s], (uint32_t)(((j >> 1) & 1) ^ 1), a.timeout_ns)) return false;
+        tc_fence_after();
+        const uint32_t sk = slot(u);
+#pragma unroll
+        for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int pl = 0; pl < 2; ++pl)
+              mma_f8f6f4_ss(tbase + S_COL + s * KT, sdesc_k_sw128(sq + pl * C::PLANE_Q + h * (ROWS * 128) + 32 * k),
+                            sdesc_k_sw128(sk + h * (KT * 128) + 32 * k), idesc_s, (h > 0 || k > 0 || pl > 0) ? 1u : 0u);
+        tc_commit(&s_full[s]);
+        tc_commit(&empty[u % C::SLOTS]);
+        return true;
+      };
+      if (ok) ok = issue_s(0);
+      for (int j = 0; ok && j < n; ++j) {
+        if (j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
+        const int u = unit_v(j);
+        if (!mbar_wait(p_full, (uint32_t)(j & 1), a.timeout_ns)) { ok = false; break; }
+        if (!wait_unit(u)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t sv = slot(u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int pl = 0; pl < 2; ++pl)
+            mma_f8f6f4_ss(tbase + O_COL, sdesc_k_sw128(spp + pl * C::PLANE_P + 32 * k), sdesc_mn(sv + k * 4096), idesc_o,
+                          (j > 0 || k > 0 || pl > 0) ? 1u : 0u);
+        tc_commit(pv_done);
+        tc_commit(&empty[u % C::SLOTS]);
+      }
+      if (!ok) report_error(a.status, kErrMbarTimeout, 323, 0);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    const int r = q * 32 + lane;  // TMEM lane == tile row
+    const bool valid = r < nrows;
+    const int rt = valid ? r / a.G : 0, rg = r % a.G;
+    const int tok = tok0 + rt, head = kvh * a.G + rg;
+    const int ctx = valid ? context(a, tok) : 0;
+    const int seen = a.window > 0 ? ctx - a.window : 0;  // keys from here on are in the window
+    float sl2 = a.scale_log2;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + head * D);
+      float amax = 0.f;
+      if (valid)
+        for (int c = 0; c < D / 16; ++c) {
+          const uint4 raw[2] = {src[2 * c], src[2 * c + 1]};
+          amax = fmaxf(amax, amax16(raw));
+        }
+      const int e = mx_exponent(amax, 448.f);
+      sl2 *= exp2i(max(e, -126));
+      for (int c = 0; c < D / 16; ++c) {
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+        if (valid) {
+          const uint4 raw[2] = {src[2 * c], src[2 * c + 1]};
+          split16(raw, exp2i(-e), hi, lo);
+        }
+        uint8_t* dst = smem + C::OFF_Q + (c / 8) * (ROWS * 128) + r * 128 + (((c % 8) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = hi;
+        *reinterpret_cast<uint4*>(dst + C::PLANE_Q) = lo;
+      }
+      fence_proxy_async();
+      mbar_arrive(q_full);
+    }
+    float m_ref = -INFINITY, l = 0.f;
+    const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
+    uint8_t* prow = smem + C::OFF_P + r * 128;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int s = j & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns));
+      if (!ok) break;
+      tc_fence_after();
+      float sv[KT];
+#pragma unroll
+      for (int c = 0; c < KT; c += 16) tmem_ld16(trow + S_COL + s * KT + c, sv + c);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(&s_free[s]);
+      const int key0 = sp.key0(j0 + j), end = sp.end(j0 + j);
+      const bool whole = key0 + KT <= min(ctx_min, end) && (a.window == 0 || key0 >= ctx_max - a.window);
+      float tmax = -INFINITY;
+      if (whole) {
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          sv[c] *= sl2;
+          tmax = fmaxf(tmax, sv[c]);
+        }
+      } else {
+        const int top = min(ctx, end);
+#pragma unroll
+        for (int c = 0; c < KT; ++c) {
+          const int key = key0 + c;
+          sv[c] = key < top && (key >= seen || key < a.sinks) ? sv[c] * sl2 : -INFINITY;
+          tmax = fmaxf(tmax, sv[c]);
+        }
+        const int u = unit_v(j);
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns));
+        if (!ok) break;
+        clean_value_row<D>(a, smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT, r, key0 + r, end, tok0, ntok, poison);
+      }
+      // the P planes and O are free once the PV product of the tile before is done
+      if (j > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const bool need = m_ref != -INFINITY && tmax > m_ref + P_LAG;
+      if (__any_sync(0xffffffffu, need)) {
+        const float f = need ? exp2f(m_ref - tmax) : 1.f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+          tmem_ld16(trow + O_COL + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] *= f;
+          tmem_st16(trow + O_COL + c, o);
+        }
+        tmem_st_wait();
+        l *= f;
+      }
+      if (need || m_ref == -INFINITY) m_ref = tmax;
+      const float off = m_ref == -INFINITY ? 0.f : P_SHIFT - m_ref;  // a row that has seen no key: exp2(-inf) = 0
+      float lsum = 0.f;
+#pragma unroll
+      for (int c = 0; c < KT; c += 16) {
+        uint4 hi, lo;
+        uint32_t* ph = reinterpret_cast<uint32_t*>(&hi);
+        uint32_t* pl = reinterpret_cast<uint32_t*>(&lo);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float p[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[k] = exp2f(sv[c + 4 * i + k] + off);
+          lsum += (p[0] + p[1]) + (p[2] + p[3]);
+          uint32_t h0, l0, h1, l1;
+          split2(p[0], p[1], h0, l0);
+          split2(p[2], p[3], h1, l1);
+          ph[i] = h0 | (h1 << 16);
+          pl[i] = l0 | (l1 << 16);
+        }
+        uint8_t* dst = prow + (((c / 16) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(dst) = hi;
+        *reinterpret_cast<uint4*>(dst + C::PLANE_P) = lo;
+      }
+      l += lsum;
+      fence_proxy_async();
+      tc_fence_before();
+      mbar_arrive(p_full);
+    }
+    if (ok && n > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((n - 1) & 1), a.timeout_ns));
+      tc_fence_after();
+    }
+    if (!ok) report_error(a.status, kErrMbarTimeout, 324, r);
+    const bool have = n > 0 && ok;
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // poison marks
+    if (valid && poison[rt]) l = __int_as_float(0x7fffffff);
+    if (ctx == 0) l = 0.f;  // sees nothing (its scores of whole tiles were not masked)
+    if (nsplit == 1) {
+      const float inv = have && l != 0.f ? a.v_scale / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        float o[16];
+        if (have) {
+          tmem_ld16(trow + O_COL + c, o);
+          tmem_ld_wait();
+        }
+        if (!valid) continue;
+        uint4 w[2];
+        __nv_bfloat16* we = reinterpret_cast<__nv_bfloat16*>(w);
+        uint4 gr[2] = {};
+        if (a.gate != nullptr) {
+          const uint4* g = reinterpret_cast<const uint4*>(a.gate + (int64_t)tok * a.ld_gate + head * D + c);
+          gr[0] = g[0];
+          gr[1] = g[1];
+        }
+        const __nv_bfloat16* ge = reinterpret_cast<const __nv_bfloat16*>(gr);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float v = inv != 0.f ? o[i] * inv : 0.f;  // O of a row without weights was never written
+          if (a.gate != nullptr) v *= sigmoid_f(__bfloat162float(ge[i]));
+          we[i] = __float2bfloat16(v);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(a.out + (int64_t)tok * a.ld_out + head * D + c);
+        dst[0] = w[0];
+        dst[1] = w[1];
+      }
+    } else {
+      // partial results over the ring: row r's 16-byte pieces at c ^ (r & 31), so that a warp's
+      // stores spread over the banks
+      float* part = reinterpret_cast<float*>(smem + C::OFF_RING) + r * D;
+#pragma unroll 1
+      for (int c = 0; c < D && have; c += 16) {
+        float o[16];
+        tmem_ld16(trow + O_COL + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<float4*>(part + (((c / 4 + i) ^ (r & 31)) << 2)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      }
+      row_m[r] = have ? m_ref : -INFINITY;
+      row_l[r] = have ? l : 0.f;
+    }
+  }
+  tc_fence_before();
+  if (nsplit > 1) {
+    cluster_sync();
+    // rows r = split, split + nsplit, ...: a warp a row, a lane four dims at a time
+    const uint32_t part = smem_u32(smem + C::OFF_RING), ml = smem_u32(row_m);
+    for (int r = split + nsplit * warp; r < nrows; r += nsplit * (THREADS / 32)) {
+      const float m_l = lane < nsplit ? ld_dsmem(mapa_shared(ml, (uint32_t)lane) + r * 4) : -INFINITY;
+      const float l_l = lane < nsplit ? ld_dsmem(mapa_shared(ml, (uint32_t)lane) + (ROWS + r) * 4) : 0.f;
+      float M = l_l != 0.f ? m_l : -INFINITY;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      const float w_l = l_l == 0.f ? 0.f : m_l == -INFINITY ? 1.f : exp2f(m_l - M);
+      float L = l_l == 0.f ? 0.f : w_l * l_l;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      const float inv = L != 0.f ? a.v_scale / L : 0.f;
+      const int tok = tok0 + r / a.G, head = kvh * a.G + r % a.G;
+      for (int c = lane; c < D / 4; c += 32) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < nsplit; ++s) {
+          const float w = __shfl_sync(0xffffffffu, w_l, s);
+          const float4 v = ld_dsmem_f4(mapa_shared(part, (uint32_t)s) + (r * D + ((c ^ (r & 31)) << 2)) * 4);
+          if (w != 0.f) {
+            acc.x += w * v.x;
+            acc.y += w * v.y;
+            acc.z += w * v.z;
+            acc.w += w * v.w;
+          }
+        }
+        float o[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+        const int64_t col = (int64_t)head * D + 4 * c;
+        uint2 w2;
+        __nv_bfloat16* we = reinterpret_cast<__nv_bfloat16*>(&w2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (a.gate != nullptr) o[i] *= sigmoid_f(__bfloat162float(a.gate[(int64_t)tok * a.ld_gate + col + i]));
+          we[i] = __float2bfloat16(o[i]);
+        }
+        *reinterpret_cast<uint2*>(a.out + (int64_t)tok * a.ld_out + col) = w2;
+      }
+    }
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, C::TMEM_COLS);
+  }
+}
+
+template <typename K>
+static void launch_cluster(K kern, int smem, dim3 grid, int threads, const CUtensorMap& tk, const CUtensorMap& tv, const wa::Args& a) {
+  TORCH_CHECK(ensure_smem_attr((const void*)kern, smem) == cudaSuccess, "window_attention: shared memory attribute");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = at::cuda::getCurrentCUDAStream();
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {1, 1, grid.z};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  TORCH_CHECK(cudaLaunchKernelEx(&cfg, kern, tk, tv, a) == cudaSuccess, "window_attention launch");
 }
 
 void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_table,
@@ -144,7 +1081,6 @@ void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
               "window_attention: sizes out of range");
   if (T == 0 || S == 0) return;
   const at::cuda::CUDAGuard guard(q.device());
-  auto st = at::cuda::getCurrentCUDAStream();
   wa::Args a = {};
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
   a.ld_q = q.stride(0);
@@ -170,12 +1106,38 @@ void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
   a.window = (int)window;
   a.sinks = window > 0 ? (int)sinks : 0;
   a.max_new = (int)std::min(max_new, T);
-  a.scale = (float)(sm_scale * k_scale);
   a.v_scale = (float)v_scale;
   a.status = status.data_ptr<int>();
-  const dim3 grid((unsigned)a.max_new, (unsigned)((Hq + 3) / 4), (unsigned)S);
-  TORCH_CHECK(launch_pdl(D == 128 ? window_attn_simple_kernel<128> : window_attn_simple_kernel<256>, grid, dim3(128), 0, st,
-                         a) == cudaSuccess, "window_attention launch");
+  a.scale_log2 = (float)(sm_scale * k_scale * 1.4426950408889634);
+  a.timeout_ns = 1000000000ull;
+  const CUtensorMap tk = tmap_u8_kmajor(k_cache.data_ptr(), k_cache.size(0) * Hkv * wa::PAGE, D, wa::PAGE);
+  const CUtensorMap tv = tmap_u8_kmajor(v_cache.data_ptr(), v_cache.size(0) * Hkv * wa::PAGE, D, wa::PAGE);
+  // tiles of keys that one group of rows can see at most
+  const int64_t span = window > 0 ? std::min(max_ctx, window + sinks + a.max_new + 2 * wa::KT) : max_ctx;
+  const int64_t tiles = (span + wa::KT - 1) / wa::KT;
+  const int64_t sms = device_sm_count();
+  const int64_t nq = (int64_t)a.max_new * a.G;  // rows of the longest sequence and one kv head
+  const bool dec = nq <= wd::N;
+  const int64_t per = wc::ROWS / a.G;
+  const int64_t groups = dec ? S : std::min(T / per + S, S * ((a.max_new + per - 1) / per));
+  // CTAs of a cluster share a group's keys while that fills the GPU and leaves each of them a tile
+  int64_t nsplit = 1;
+  while (nsplit < 8 && groups * Hkv * nsplit * 2 <= sms * (dec ? 2 : 1) && nsplit * 2 <= tiles) nsplit *= 2;
+  const dim3 grid((unsigned)groups, (unsigned)Hkv, (unsigned)nsplit);
+  TORCH_CHECK(groups <= INT_MAX, "window_attention: too many rows");
+  if (dec) {
+    if (D == 128) {
+      if (nq <= 8) launch_cluster(window_attn_dec_kernel<128, 8>, wd::Cfg<128>::SMEM, grid, wd::THREADS, tk, tv, a);
+      else launch_cluster(window_attn_dec_kernel<128, 16>, wd::Cfg<128>::SMEM, grid, wd::THREADS, tk, tv, a);
+    } else {
+      if (nq <= 8) launch_cluster(window_attn_dec_kernel<256, 8>, wd::Cfg<256>::SMEM, grid, wd::THREADS, tk, tv, a);
+      else launch_cluster(window_attn_dec_kernel<256, 16>, wd::Cfg<256>::SMEM, grid, wd::THREADS, tk, tv, a);
+    }
+  } else if (D == 128) {
+    launch_cluster(window_attn_chunk_kernel<128>, wc::Cfg<128>::SMEM, grid, wc::THREADS, tk, tv, a);
+  } else {
+    launch_cluster(window_attn_chunk_kernel<256>, wc::Cfg<256>::SMEM, grid, wc::THREADS, tk, tv, a);
+  }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
