@@ -10,12 +10,20 @@
 // one (finer than the 2^-24 steps of the uniform number itself), so every sum is exact: the token
 // depends on the row and its number alone, not on the order of additions, the batch or the launch.
 //
-// A row belongs to a cluster of CTAs. Each holds a slice of it in shared memory, so the logits are
-// read from memory once; the CTAs exchange a few numbers a round through distributed shared memory.
-// Both cuts are of the form "the smallest key B with F(keys <= B) >= target", F = count or weight.
+// A row belongs to a cluster of CTAs; each holds a slice of it in shared memory, so the logits are read
+// from memory once. Both cuts look for "the smallest key B with F(keys <= B) >= target", F = count or
+// weight, keys ordered as above:
+//   * a histogram of (m - x) / T over 1024 bins a CTA (shared-memory atomics on whole numbers), summed by
+//     the cluster's first CTA, gives the bin in which F crosses the target;
+//   * if all keys up to that bin are few (top-k and most nuclei), they go to the first CTA, which sorts
+//     them, applies all three filters and draws; the other CTAs are done;
+//   * else the crossing bin's keys are sorted there (after a second, 1024 times finer histogram if they
+//     are many; bit by bit over the cluster if thousands tie), and the cut key goes back to all CTAs,
+//     which sum and draw over their slices.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <climits>
 #include "common.cuh"
 
 namespace r9k {
@@ -24,7 +32,12 @@ namespace sm {
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 16;
-constexpr float ONE = 2147483648.f;  // 2^31
+constexpr int BINS = 2 * THREADS;
+constexpr int CAP = 2 * THREADS;         // keys that one CTA sorts: two a thread
+constexpr float ONE = 2147483648.f;      // 2^31
+constexpr float REACH = 21.6f;           // exp(-z) 2^31 < 1 beyond: no weight
+constexpr int WORK_BYTES = 3 * BINS * 4;  // histograms (count, low and high half of the weights), or the list
+static_assert(CAP * 8 <= WORK_BYTES, "the list lies over the histograms");
 
 struct Args {
   const void* logits;
@@ -39,78 +52,242 @@ struct Args {
   float* logprobs;
 };
 
-// one number of each CTA of the cluster, two rounds deep (a round's slots are written again two
-// rounds later, when every CTA has passed the barrier after its reads)
-struct Shared {
-  unsigned long long slot[2];
-  unsigned long long warp[WARPS];
-  unsigned long long result[2];
+using u64 = unsigned long long;
+
+enum Op { SUM, MAX };
+enum Action { DONE, FINISH, CUT, REFINE, BITS };
+
+struct Verdict {  // of the first CTA, sent to all
+  u64 target, before;
+  int action, bin;
 };
 
-R9K_DEVINL unsigned long long ld_dsmem_u64(uint32_t addr) {
-  unsigned long long v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+struct Shared {
+  u64 slot[2][MAX_CLUSTER];  // one number of each CTA, two rounds deep
+  u64 warp[WARPS];
+  u64 warp2[WARPS];
+  u64 last;
+  Verdict verdict;
+  uint32_t listed;
+};
+
+R9K_DEVINL void st_dsmem(uint32_t addr, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
+R9K_DEVINL uint2 ld_dsmem_u2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
-
-R9K_DEVINL float load_logit(const Args& a, int64_t i, float) { return reinterpret_cast<const float*>(a.logits)[i]; }
-R9K_DEVINL float load_logit(const Args& a, int64_t i, __nv_bfloat16) {
-  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.logits)[i]);
+R9K_DEVINL uint32_t add_dsmem(uint32_t addr, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
+  return old;
 }
+R9K_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+R9K_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // larger x -> smaller key (x is not NaN, and -0 counts as 0)
 R9K_DEVINL uint32_t order_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? b : ~(b | 0x80000000u);
 }
+R9K_DEVINL float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k : ~k & 0x7fffffffu); }
+R9K_DEVINL u64 full_key(float x, int i) { return ((u64)order_key(x) << 32) | (uint32_t)i; }
 
 struct Row {
-  float m, inv_t, min_p;
+  float m, inv_t, min_p, p, bins;  // bins: histogram bins of one unit of (m - x) / T
+  int k;
   R9K_DEVINL float e(float x) const {
     if (x == m) return 1.f;
     if (!(x > -INFINITY)) return 0.f;
     return expf((x - m) * inv_t);
   }
   R9K_DEVINL uint32_t w(float x) const { return (uint32_t)(e(x) * ONE); }
+  // place in the histogram, ascending in the order of keys; >= BINS: no weight (NaN does not compare).
+  // Every use has to round alike, so the products are not to be fused with what follows.
+  R9K_DEVINL float place(float x) const { return x == m ? 0.f : __fmul_rn(__fmul_rn(m - x, inv_t), bins); }
 };
 
-enum Op { SUM, MAX };
+R9K_DEVINL u64 join(u64 a, u64 b, Op op) { return op == SUM ? a + b : (a > b ? a : b); }
 
-R9K_DEVINL unsigned long long join(unsigned long long a, unsigned long long b, Op op) {
-  return op == SUM ? a + b : (a > b ? a : b);
-}
-
-// The cluster's sum or maximum of v, in every thread; own: this CTA's; before: of the CTAs before it
-R9K_DEVINL unsigned long long cluster_join(unsigned long long v, Op op, Shared* s, int& round, unsigned long long* before) {
+// The cluster's sum or maximum of v, in every thread; before: the sum over the CTAs before this one.
+// Every CTA writes its number to all others; a round's slots are written again two rounds later, after
+// a barrier that comes after everybody's reads.
+R9K_DEVINL u64 cluster_join(u64 v, Op op, Shared* s, int& round, u64* before) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = (int)cluster_nctarank(), me = (int)cluster_ctarank();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o), op);
   if (lane == 0) s->warp[warp] = v;
   __syncthreads();
+  u64* slot = s->slot[round & 1];
   if (warp == 0) {
-    unsigned long long t = lane < WARPS ? s->warp[lane] : 0ull;
+    u64 t = lane < WARPS ? s->warp[lane] : 0ull;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = join(t, __shfl_xor_sync(0xffffffffu, t, o), op);
-    if (lane == 0) s->slot[round & 1] = t;
+    if (lane < n) st_dsmem(mapa_shared(smem_u32(&slot[me]), (uint32_t)lane), t);
   }
   cluster_sync();
-  if (warp == 0) {
-    const int n = (int)cluster_nctarank(), me = (int)cluster_ctarank();
-    unsigned long long t = lane < n ? ld_dsmem_u64(mapa_shared(smem_u32(&s->slot[round & 1]), (uint32_t)lane)) : 0ull;
-    unsigned long long b = lane < me ? t : 0ull;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      t = join(t, __shfl_xor_sync(0xffffffffu, t, o), op);
-      b = join(b, __shfl_xor_sync(0xffffffffu, b, o), op);
-    }
-    if (lane == 0) { s->result[0] = t; s->result[1] = b; }
+  u64 t = 0, b = 0;
+  for (int i = 0; i < n; ++i) {
+    if (i == me) b = t;
+    t = join(t, slot[i], op);
   }
-  __syncthreads();
   ++round;
-  const unsigned long long r = s->result[0];
-  if (before != nullptr) *before = s->result[1];
+  if (before != nullptr) *before = b;
+  return t;
+}
+
+// inclusive sums over the block; total: of all threads
+R9K_DEVINL u64 block_scan(u64 v, u64* scratch, u64* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  if (lane == 31) scratch[warp] = v;
   __syncthreads();
-  return r;
+  u64 t = lane < WARPS ? scratch[lane] : 0ull;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, t, o);
+    if (lane >= o) t += x;
+  }
+  *total = __shfl_sync(0xffffffffu, t, 31);
+  const u64 pre = __shfl_sync(0xffffffffu, t, (warp + 31) & 31);
+  __syncthreads();
+  return v + (warp > 0 ? pre : 0ull);
+}
+
+// Ascending sort of two numbers a thread (places t and t + THREADS) of which the first n matter; the
+// others are ~0. Neighbours nearer than a warp exchange by shuffles, further ones through buf [CAP].
+R9K_DEVINL void block_sort(u64 (&v)[2], int n, u64* buf) {
+  const int t = threadIdx.x;
+  const bool two = n > THREADS;
+  for (int size = 2; size < 2 * n; size <<= 1) {
+    for (int j = size >> 1; j > 0; j >>= 1) {
+      if (j == THREADS) {
+        const u64 a = v[0], b = v[1];
+        v[0] = a < b ? a : b;
+        v[1] = a < b ? b : a;
+        continue;
+      }
+      u64 o[2] = {~0ull, ~0ull};
+      if (j >= 32) {
+        buf[t] = v[0];
+        if (two) buf[t + THREADS] = v[1];
+        __syncthreads();
+        o[0] = buf[t ^ j];
+        if (two) o[1] = buf[(t ^ j) + THREADS];
+        __syncthreads();
+      } else {
+        o[0] = __shfl_xor_sync(0xffffffffu, v[0], j);
+        if (two) o[1] = __shfl_xor_sync(0xffffffffu, v[1], j);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = t + i * THREADS;
+        const bool low = ((at & j) == 0) == ((at & size) == 0);
+        v[i] = low == (v[i] < o[i]) ? v[i] : o[i];
+      }
+    }
+  }
+}
+
+template <typename T>
+R9K_DEVINL float as_logit(T v);
+template <>
+R9K_DEVINL float as_logit(float v) { return v != v ? -INFINITY : v; }
+template <>
+R9K_DEVINL float as_logit(__nv_bfloat16 v) { return as_logit(__bfloat162float(v)); }
+
+// The slice's n logits to shared memory as fp32, largest and smallest (finite) on the way: 16-byte
+// loads from the first such boundary on. Returns where they begin (the stores keep the loads' alignment).
+template <typename T>
+R9K_DEVINL const float* load_slice(const T* src, int n, float* buf, float& hi, float& lo) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
+  float* xs = buf + ((4 - (head & 3)) & 3);
+  auto see = [&](float x) {
+    hi = fmaxf(hi, x);
+    if (x > -INFINITY) lo = fminf(lo, x);
+  };
+  const int vecs = (n - head) / VEC;
+  const uint4* body = reinterpret_cast<const uint4*>(src + head);
+#pragma unroll 8
+  for (int v = threadIdx.x; v < vecs; v += THREADS) {
+    const uint4 raw = body[v];
+    const T* e = reinterpret_cast<const T*>(&raw);
+    float x[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      x[i] = as_logit(e[i]);
+      see(x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4)
+      *reinterpret_cast<float4*>(xs + head + v * VEC + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  }
+  const int rest = head + vecs * VEC;
+  for (int i = threadIdx.x; i < head + n - rest; i += THREADS) {
+    const int at = i < head ? i : rest + i - head;
+    const float x = as_logit(src[at]);
+    see(x);
+    xs[at] = x;
+  }
+  return xs;
+}
+
+// The first CTA's last step: the keys up to the cut, sorted; all filters; the draw in index order.
+// all: the weight that top-p is a share of (0: that of the first k keys).
+R9K_DEVINL void finish_list(const Args& a, const Row& r, int row, int n, u64 all, u64* list, Shared* s) {
+  const int t = threadIdx.x;
+  u64 v[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] = t + i * THREADS < n ? list[t + i * THREADS] : ~0ull;
+  __syncthreads();
+  block_sort(v, n, list);
+  const int k = r.k > 0 ? min(r.k, n) : n;
+  u64 w[2], upto[2], total = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = t + i * THREADS < k ? r.w(key_value((uint32_t)(v[i] >> 32))) : 0ull;
+    u64 part;
+    upto[i] = total + block_scan(w[i], s->warp, &part);
+    total += part;
+  }
+  if (all == 0) all = total;
+  const double enough = (double)r.p * (double)all;
+  int kept = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = t + i * THREADS;
+    const bool keep = at < k && (at == 0 || !(r.p < 1.f) || (double)(upto[i] - w[i]) < enough) &&
+                      r.e(key_value((uint32_t)(v[i] >> 32))) >= r.min_p;
+    kept += keep;
+    v[i] = keep ? (v[i] << 32) | w[i] : ~0ull;  // now by index
+  }
+  // the kept keys are the first ones: how many
+  u64 count;
+  block_scan((u64)kept, s->warp, &count);
+  block_sort(v, (int)count, list);
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = v[i] == ~0ull ? 0ull : (uint32_t)v[i];
+    u64 part;
+    upto[i] = total + block_scan(w[i], s->warp, &part);
+    total += part;
+  }
+  const double at = floor((double)a.u[row] * (double)total);
+  u64 target = at > 0. ? (u64)at : 0ull;  // a NaN draws the first
+  if (target > total - 1) target = total - 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (upto[i] - w[i] <= target && target < upto[i]) {
+      a.tokens[row] = (int64_t)(v[i] >> 32);
+      a.logprobs[row] = (float)log((double)w[i] / (double)total);
+    }
 }
 }  // namespace sm
 
@@ -119,118 +296,231 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
   using namespace sm;
   pdl_wait();
   pdl_trigger();
-  extern __shared__ float xs[];  // this CTA's slice of the row
+  cluster_arrive();  // every CTA runs before its shared memory is written to (waited for below)
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
+  uint32_t* count = reinterpret_cast<uint32_t*>(smem);  // histograms
+  uint32_t* wlow = count + BINS;
+  uint32_t* whigh = wlow + BINS;
+  u64* list = reinterpret_cast<u64*>(smem);  // the first CTA's, after the histograms
+  float* buf = reinterpret_cast<float*>(smem + WORK_BYTES);
   const int n_cta = (int)cluster_nctarank(), me = (int)cluster_ctarank();
   const int row = blockIdx.x / n_cta;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int i0 = me * a.slice;
   const int n = max(0, min(a.V - i0, a.slice));
   int round = 0;
 
-  // the row's maximum and its lowest index
-  unsigned long long best = 0;
-  for (int i = tid; i < n; i += THREADS) {
-    float x = load_logit(a, (int64_t)row * a.ld + i0 + i, T());
-    if (x != x) x = -INFINITY;
-    xs[i] = x;
-    const unsigned long long k = ((unsigned long long)~order_key(x) << 32) | (uint32_t)~(i0 + i);
-    best = best > k ? best : k;
-  }
-  best = cluster_join(best, MAX, &sh, round, nullptr);  // its barriers make the slice visible too
-  const int arg = (int)~(uint32_t)best;
-  const uint32_t kmax = ~(uint32_t)(best >> 32);
+  float hi = -INFINITY, lo = INFINITY;
+  const float* xs = load_slice(reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.ld + i0, n, buf, hi, lo);
+  cluster_wait();
+  // the maximum of ~key is the maximum; that of a key is the smallest value. 32 bits each
+  const u64 top = cluster_join(((u64)(uint32_t)~order_key(hi) << 32), MAX, &sh, round, nullptr);
   Row r;
-  r.m = __uint_as_float((kmax & 0x80000000u) ? kmax : ~kmax & 0x7fffffffu);
+  r.m = key_value(~(uint32_t)(top >> 32));
   const float t = a.temperature[row];
-  if (!(t > 0.f) || r.m == -INFINITY) {  // greedy; a row with nothing to draw from has no token
+  if (r.m == -INFINITY) {  // nothing to draw from
     if (me == 0 && tid == 0) {
-      a.tokens[row] = r.m == -INFINITY ? -1 : arg;
-      a.logprobs[row] = r.m == -INFINITY ? -INFINITY : 0.f;
+      a.tokens[row] = -1;
+      a.logprobs[row] = -INFINITY;
     }
-    cluster_sync();
+    return;
+  }
+  if (!(t > 0.f)) {
+    uint32_t best = 0;  // ~index
+    for (int i = tid; i < n; i += THREADS)
+      if (xs[i] == r.m) {
+        best = ~(uint32_t)(i0 + i);
+        break;
+      }
+    const u64 first = cluster_join((u64)best, MAX, &sh, round, nullptr);
+    if (me == 0 && tid == 0) {
+      a.tokens[row] = (int64_t)(uint32_t)~(uint32_t)first;
+      a.logprobs[row] = 0.f;
+    }
     return;
   }
   r.inv_t = 1.f / t;
   r.min_p = a.min_p ? fminf(fmaxf(a.min_p[row], 0.f), 1.f) : 0.f;
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.f;
+  r.k = a.top_k ? a.top_k[row] : 0;
+  if (r.k < 0 || r.k >= a.V) r.k = 0;
+  r.p = a.top_p ? a.top_p[row] : 1.f;
+  if (!(r.p < 1.f)) r.p = 1.f;
+  const bool cuts[2] = {r.k > 0, r.p < 1.f};
 
-  // last kept key of the order, as (key, index); all bits set: everything
-  unsigned long long last = ~0ull;
+  u64 last = ~0ull;  // last kept key
+  if (cuts[0] || cuts[1]) {
+    // bins over what the row spans, where that is less than the weights' reach (high temperatures)
+    const u64 bottom = cluster_join(lo < INFINITY ? (u64)order_key(lo) : 0ull, MAX, &sh, round, nullptr);
+    const float span = fminf(REACH, (r.m - key_value((uint32_t)bottom)) * r.inv_t * 1.001f);
+    r.bins = span > 1e-6f ? (float)BINS / span : (float)BINS * 1e6f;  // infinities: span = REACH
+  }
   for (int cut = 0; cut < 2; ++cut) {
-    if (cut == 0 ? !(k > 0 && k < a.V) : !(p < 1.f)) continue;
-    unsigned long long target = (unsigned long long)k;
-    if (cut == 1) {
-      unsigned long long sum = 0;
+    if (!cuts[cut]) continue;
+    float cell = 0.f, fine = 1.f;  // the histogram covers places [cell, cell + BINS / fine)
+    u64 target = (u64)r.k, before = 0;
+    for (int level = 0;; ++level) {
+      for (int i = tid; i < (cut == 0 ? BINS : 3 * BINS); i += THREADS) count[i] = 0;
+      if (tid == 0) sh.listed = 0;
+      __syncthreads();
       for (int i = tid; i < n; i += THREADS) {
-        const unsigned long long key = ((unsigned long long)order_key(xs[i]) << 32) | (uint32_t)(i0 + i);
-        if (key <= last) sum += r.w(xs[i]);
+        const float x = xs[i];
+        const float at = (r.place(x) - cell) * fine;
+        if (at >= 0.f && at < (float)BINS && full_key(x, i0 + i) <= last) {
+          const int bin = (int)at;
+          atomicAdd(&count[bin], 1u);
+          if (cut == 1) {  // 2^31 a weight, 2^16 weights a CTA at most: the halves' sums fit 32 bits
+            const uint32_t w = r.w(x);
+            atomicAdd(&wlow[bin], w & 0xffffu);
+            atomicAdd(&whigh[bin], w >> 16);
+          }
+        }
       }
-      sum = cluster_join(sum, SUM, &sh, round, nullptr);
-      // B_i < p P of whole numbers: the cut is the first key whose running sum reaches ceil(p P)
-      target = (unsigned long long)max(1ll, (long long)ceil((double)p * (double)sum));
-    }
-    unsigned long long lo = 0;  // F(keys < lo) < target
-    for (int bit = 63; bit >= 0; --bit) {
-      if (bit < 32 && (1ll << bit) >= 2ll * a.V) continue;  // no index has this bit
-      const unsigned long long trial = lo | (1ull << bit);
-      unsigned long long f = 0;
-      for (int i = tid; i < n; i += THREADS) {
-        const unsigned long long key = ((unsigned long long)order_key(xs[i]) << 32) | (uint32_t)(i0 + i);
-        if (key < trial && key <= last) f += cut == 0 ? 1u : r.w(xs[i]);
+      cluster_sync();
+      if (me == 0) {
+        u64 c[2] = {0, 0}, f[2] = {0, 0};  // this thread's two bins
+        for (int i = 0; i < n_cta; ++i) {
+          const uint32_t at = mapa_shared(smem_u32(&count[2 * tid]), (uint32_t)i);
+          const uint2 v = ld_dsmem_u2(at);
+          c[0] += v.x;
+          c[1] += v.y;
+          if (cut == 1) {
+            const uint2 l = ld_dsmem_u2(at + BINS * 4), h = ld_dsmem_u2(at + 2 * BINS * 4);
+            f[0] += ((u64)h.x << 16) + l.x;
+            f[1] += ((u64)h.y << 16) + l.y;
+          }
+        }
+        if (cut == 0) {
+          f[0] = c[0];
+          f[1] = c[1];
+        }
+        u64 all, keys;
+        const u64 upto = block_scan(f[0] + f[1], sh.warp, &all);
+        const u64 cupto = block_scan(c[0] + c[1], sh.warp2, &keys);
+        if (level == 0 && cut == 1) target = (u64)max(1ll, (long long)ceil((double)r.p * (double)all));
+        if (tid == 0) sh.verdict = Verdict{target, 0, keys <= CAP ? FINISH : DONE, BINS - 1};  // fewer than k keys have weight
+        __syncthreads();
+        const u64 want = target - before;
+        const u64 b0 = upto - f[0] - f[1], b1 = upto - f[1];
+        const int hit = b0 < want && want <= b1 ? 0 : b1 < want && want <= upto ? 1 : -1;
+        if (hit >= 0) {
+          const u64 through = cupto - (hit == 0 ? c[1] : 0ull);  // keys up to and with the bin
+          Verdict v{target, before + (hit == 0 ? b0 : b1), BITS, 2 * tid + hit};
+          if (level == 0 && through <= CAP) v.action = FINISH;
+          else if (c[hit] <= CAP) v.action = CUT;
+          else if (level == 0) v.action = REFINE;
+          sh.verdict = v;
+        }
+        __syncthreads();
+        if (tid == 0 && level == 0 && cut == 1) sh.last = all;
+        if (tid > 0 && tid < n_cta) {
+          const u64* from = reinterpret_cast<const u64*>(&sh.verdict);
+#pragma unroll
+          for (int i = 0; i < (int)(sizeof(Verdict) / 8); ++i)
+            st_dsmem(mapa_shared(smem_u32(&sh.verdict), (uint32_t)tid) + 8 * i, from[i]);
+        }
       }
-      f = cluster_join(f, SUM, &sh, round, nullptr);
-      if (f < target) lo = trial;
+      cluster_sync();
+      const Verdict v = sh.verdict;
+      target = v.target;
+      before = v.before;
+      if (v.action == DONE) break;
+      if (v.action == REFINE) {
+        cell = (float)v.bin;
+        fine = (float)BINS;
+        continue;
+      }
+      // the crossing bin in places: [from, to)
+      const float from = cell + (float)v.bin / fine, to = cell + (float)(v.bin + 1) / fine;
+      if (v.action == BITS) {
+        u64 low = 0;  // F(keys < low) < target
+        for (int bit = 63; bit >= 0; --bit) {
+          if (bit < 32 && (1ll << bit) >= 2ll * a.V) continue;  // no index has this bit
+          const u64 trial = low | (1ull << bit);
+          u64 f = 0;
+          for (int i = tid; i < n; i += THREADS) {
+            const float x = xs[i], at = r.place(x);
+            const u64 key = full_key(x, i0 + i);
+            if (at >= from && at < to && key < trial && key <= last) f += cut == 0 ? 1u : r.w(x);
+          }
+          f = cluster_join(f, SUM, &sh, round, nullptr);
+          if (before + f < target) low = trial;
+        }
+        last = low;
+        break;
+      }
+      // FINISH: every key up to the bin; CUT: the bin's
+      const bool finish = v.action == FINISH;
+      const uint32_t counter = mapa_shared(smem_u32(&sh.listed), 0u), dst = mapa_shared(smem_u32(list), 0u);
+      for (int i = tid - lane; i < n; i += THREADS) {
+        const bool in = i + lane < n;
+        const float x = in ? xs[i + lane] : 0.f;
+        const float at = in ? r.place(x) : INFINITY;
+        const u64 key = full_key(x, i0 + i + lane);
+        const bool take = at < to && (finish || at >= from) && key <= last;
+        const uint32_t takers = __ballot_sync(0xffffffffu, take);
+        if (takers == 0) continue;
+        uint32_t base = 0;
+        if (lane == 0) base = add_dsmem(counter, (uint32_t)__popc(takers));
+        base = __shfl_sync(0xffffffffu, base, 0) + (uint32_t)__popc(takers & ((1u << lane) - 1));
+        if (take && base < CAP) st_dsmem(dst + base * 8, key);
+      }
+      cluster_sync();
+      if (finish) {
+        if (me == 0) finish_list(a, r, row, min((int)sh.listed, CAP), cut == 1 ? sh.last : 0ull, list, &sh);
+        return;
+      }
+      if (me == 0) {
+        const int m = min((int)sh.listed, CAP);
+        u64 k2[2], total = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) k2[i] = tid + i * THREADS < m ? list[tid + i * THREADS] : ~0ull;
+        __syncthreads();
+        block_sort(k2, m, list);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u64 w = tid + i * THREADS >= m ? 0ull : cut == 0 ? 1ull : r.w(key_value((uint32_t)(k2[i] >> 32)));
+          u64 part;
+          const u64 upto = before + total + block_scan(w, sh.warp, &part);
+          total += part;
+          if (upto - w < target && target <= upto) sh.last = k2[i];
+        }
+        __syncthreads();
+        if (tid > 0 && tid < n_cta) st_dsmem(mapa_shared(smem_u32(&sh.last), (uint32_t)tid), sh.last);
+      }
+      cluster_sync();
+      last = sh.last;
+      break;
     }
-    last = lo;
   }
 
-  // weights of the kept tokens; the draw in index order
-  unsigned long long sum = 0;
+  // weights of the kept tokens, a slice a CTA; the draw in index order
+  u64 sum = 0;
   for (int i = tid; i < n; i += THREADS) {
     const float x = xs[i];
-    const unsigned long long key = ((unsigned long long)order_key(x) << 32) | (uint32_t)(i0 + i);
-    if (key <= last && r.e(x) >= r.min_p) sum += r.w(x);
+    if (full_key(x, i0 + i) <= last && r.e(x) >= r.min_p) sum += r.w(x);
   }
-  unsigned long long before;
-  const unsigned long long total = cluster_join(sum, SUM, &sh, round, &before);
+  u64 base;
+  const u64 total = cluster_join(sum, SUM, &sh, round, &base);
   const double at = floor((double)a.u[row] * (double)total);
-  unsigned long long target = at > 0. ? (unsigned long long)at : 0ull;  // a NaN draws the first
+  u64 target = at > 0. ? (u64)at : 0ull;  // a NaN draws the first
   if (target > total - 1) target = total - 1;
-  // running sums of 512 indexes at a time
-  unsigned long long base = before;
-  for (int c = 0; c < n; c += THREADS) {
+  if (target < base) return;
+  for (int c = 0; c < n && base <= target; c += THREADS) {  // running sums of 512 indexes at a time
     const int i = c + tid;
-    uint32_t w = 0;
+    u64 w = 0;
     if (i < n) {
       const float x = xs[i];
-      const unsigned long long key = ((unsigned long long)order_key(x) << 32) | (uint32_t)(i0 + i);
-      if (key <= last && r.e(x) >= r.min_p) w = r.w(x);
+      if (full_key(x, i0 + i) <= last && r.e(x) >= r.min_p) w = r.w(x);
     }
-    const int lane = tid & 31, warp = tid >> 5;
-    unsigned long long inc = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) sh.warp[warp] = inc;
-    __syncthreads();
-    unsigned long long pre = base, all = 0;
-    for (int j = 0; j < WARPS; ++j) {
-      if (j < warp) pre += sh.warp[j];
-      all += sh.warp[j];
-    }
-    if (w > 0 && pre + inc - w <= target && target < pre + inc) {
+    u64 all;
+    const u64 upto = base + block_scan(w, sh.warp, &all);
+    if (upto - w <= target && target < upto) {
       a.tokens[row] = i0 + i;
       a.logprobs[row] = (float)log((double)w / (double)total);
     }
     base += all;
-    __syncthreads();
-    if (base > target) break;
   }
-  cluster_sync();  // peers may still read this CTA's slots
 }
 
 void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperature, c10::optional<torch::Tensor> top_k,
@@ -251,7 +541,7 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   if (min_p.has_value()) chk(*min_p, torch::kFloat32, "min_p");
   chk(tokens, torch::kInt64, "tokens");
   chk(logprobs, torch::kFloat32, "logprobs");
-  constexpr int MAX_SLICE = 55 * 1024;  // floats of shared memory
+  constexpr int MAX_SLICE = 48 * 1024;  // floats of shared memory
   TORCH_CHECK(V <= (int64_t)sm::MAX_CLUSTER * MAX_SLICE, "sample_logits: vocabulary too large");
   if (R == 0) return;
   const at::cuda::CUDAGuard guard(logits.device());
@@ -264,13 +554,13 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
              min_p.has_value() ? min_p->data_ptr<float>() : nullptr, tokens.data_ptr<int64_t>(),
              logprobs.data_ptr<float>()};
   auto kern = logits.dtype() == torch::kFloat32 ? sample_kernel<float> : sample_kernel<__nv_bfloat16>;
-  TORCH_CHECK(ensure_smem_attr((const void*)kern, MAX_SLICE * 4) == cudaSuccess, "sample_logits: shared memory attribute");
+  TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + MAX_SLICE * 4 + 16) == cudaSuccess, "sample_logits: shared memory attribute");
   TORCH_CHECK(cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess,
               "sample_logits: cluster attribute");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(R * C));
   cfg.blockDim = dim3(sm::THREADS);
-  cfg.dynamicSmemBytes = (size_t)a.slice * 4;
+  cfg.dynamicSmemBytes = (size_t)sm::WORK_BYTES + (size_t)a.slice * 4 + 16;
   cfg.stream = at::cuda::getCurrentCUDAStream();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
