@@ -14,7 +14,9 @@
 // from memory once. Both cuts look for "the smallest key B with F(keys <= B) >= target", F = count or
 // weight, keys ordered as above:
 //   * a histogram of (m - x) / T over 1024 bins a CTA (shared-memory atomics on whole numbers), summed by
-//     the cluster's first CTA, gives the bin in which F crosses the target;
+//     the cluster's first CTA, gives the bin in which F crosses the target. Top-k first tries the
+//     threads' maxima alone: at least k keys lie at or before the k-th of them, and hardly more than k
+//     where k is well below the number of threads, so one atomic a thread does instead of one a key;
 //   * if all keys up to that bin are few (top-k and most nuclei), they go to the first CTA, which sorts
 //     them, applies all three filters and draws; the other CTAs are done;
 //   * else the crossing bin's keys are sorted there (after a second, 1024 times finer histogram if they
@@ -55,7 +57,7 @@ struct Args {
 using u64 = unsigned long long;
 
 enum Op { SUM, MAX };
-enum Action { DONE, FINISH, CUT, REFINE, BITS };
+enum Action { DONE, FINISH, CUT, REFINE, BITS, KEYS };
 
 struct Verdict {  // of the first CTA, sent to all
   u64 target, before;
@@ -75,6 +77,11 @@ R9K_DEVINL void st_dsmem(uint32_t addr, u64 v) { asm volatile("st.shared::cluste
 R9K_DEVINL uint2 ld_dsmem_u2(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+R9K_DEVINL uint32_t ld_dsmem_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 R9K_DEVINL uint32_t add_dsmem(uint32_t addr, uint32_t v) {
@@ -135,6 +142,27 @@ R9K_DEVINL u64 cluster_join(u64 v, Op op, Shared* s, int& round, u64* before) {
   ++round;
   if (before != nullptr) *before = b;
   return t;
+}
+
+// the cluster's maxima of two 32-bit numbers at once
+R9K_DEVINL uint2 cluster_max2(uint32_t x, uint32_t y, Shared* s, int& round) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = (int)cluster_nctarank(), me = (int)cluster_ctarank();
+  x = __reduce_max_sync(0xffffffffu, x);
+  y = __reduce_max_sync(0xffffffffu, y);
+  if (lane == 0) s->warp[warp] = ((u64)x << 32) | y;
+  __syncthreads();
+  u64* slot = s->slot[round & 1];
+  if (warp == 0) {
+    const u64 t = lane < WARPS ? s->warp[lane] : 0ull;
+    x = __reduce_max_sync(0xffffffffu, (uint32_t)(t >> 32));
+    y = __reduce_max_sync(0xffffffffu, (uint32_t)t);
+    if (lane < n) st_dsmem(mapa_shared(smem_u32(&slot[me]), (uint32_t)lane), ((u64)x << 32) | y);
+  }
+  cluster_sync();
+  const u64 t = lane < n ? slot[lane] : 0ull;
+  ++round;
+  return make_uint2(__reduce_max_sync(0xffffffffu, (uint32_t)(t >> 32)), __reduce_max_sync(0xffffffffu, (uint32_t)t));
 }
 
 // inclusive sums over the block; total: of all threads
@@ -238,6 +266,91 @@ R9K_DEVINL const float* load_slice(const T* src, int n, float* buf, float& hi, f
   return xs;
 }
 
+// Ascending sort of 32 * E numbers of one warp, number i of lane l at place i * 32 + l.
+template <int E>
+R9K_DEVINL void warp_sort(u64 (&v)[E]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32 * E; size <<= 1) {
+#pragma unroll
+    for (int j = size >> 1; j > 0; j >>= 1) {
+      if (j >= 32) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int o = i ^ (j >> 5);
+          if (o > i) {
+            const bool up = ((i * 32) & size) == 0;
+            const u64 x = v[i], y = v[o];
+            const bool swap = (x > y) == up;
+            v[i] = swap ? y : x;
+            v[o] = swap ? x : y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const u64 o = __shfl_xor_sync(0xffffffffu, v[i], j);
+          const bool low = ((lane & j) == 0) == (((i * 32 + lane) & size) == 0);
+          v[i] = low == (v[i] < o) ? v[i] : o;
+        }
+      }
+    }
+  }
+}
+template <int E>
+R9K_DEVINL u64 warp_scan(const u64 (&w)[E], u64 (&upto)[E]) {  // inclusive; returns the total
+  const int lane = threadIdx.x & 31;
+  u64 total = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    u64 v = w[i];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += x;
+    }
+    upto[i] = total + v;
+    total += __shfl_sync(0xffffffffu, v, 31);
+  }
+  return total;
+}
+
+// finish_list() for up to 32 * E keys by one warp, without a barrier
+template <int E>
+R9K_DEVINL void finish_short(const Args& a, const Row& r, int row, int n, u64 all, const u64* list) {
+  const int lane = threadIdx.x & 31;
+  u64 v[E], w[E], upto[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = i * 32 + lane < n ? list[i * 32 + lane] : ~0ull;
+  warp_sort<E>(v);
+  const int k = r.k > 0 ? min(r.k, n) : n;
+#pragma unroll
+  for (int i = 0; i < E; ++i) w[i] = i * 32 + lane < k ? r.w(key_value((uint32_t)(v[i] >> 32))) : 0ull;
+  u64 total = warp_scan<E>(w, upto);
+  if (all == 0) all = total;
+  const double enough = (double)r.p * (double)all;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int at = i * 32 + lane;
+    const bool keep = at < k && (at == 0 || !(r.p < 1.f) || (double)(upto[i] - w[i]) < enough) &&
+                      r.e(key_value((uint32_t)(v[i] >> 32))) >= r.min_p;
+    v[i] = keep ? (v[i] << 32) | w[i] : ~0ull;  // now by index
+  }
+  warp_sort<E>(v);
+#pragma unroll
+  for (int i = 0; i < E; ++i) w[i] = v[i] == ~0ull ? 0ull : (uint32_t)v[i];
+  total = warp_scan<E>(w, upto);
+  const double at = floor((double)a.u[row] * (double)total);
+  u64 target = at > 0. ? (u64)at : 0ull;
+  if (target > total - 1) target = total - 1;
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (upto[i] - w[i] <= target && target < upto[i]) {
+      a.tokens[row] = (int64_t)(v[i] >> 32);
+      a.logprobs[row] = (float)log((double)w[i] / (double)total);
+    }
+}
+
 // The first CTA's last step: the keys up to the cut, sorted; all filters; the draw in index order.
 // all: the weight that top-p is a share of (0: that of the first k keys).
 R9K_DEVINL void finish_list(const Args& a, const Row& r, int row, int n, u64 all, u64* list, Shared* s) {
@@ -314,10 +427,10 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
   float hi = -INFINITY, lo = INFINITY;
   const float* xs = load_slice(reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.ld + i0, n, buf, hi, lo);
   cluster_wait();
-  // the maximum of ~key is the maximum; that of a key is the smallest value. 32 bits each
-  const u64 top = cluster_join(((u64)(uint32_t)~order_key(hi) << 32), MAX, &sh, round, nullptr);
+  // ~key ascends with the value, a key descends: the largest and the smallest value
+  const uint2 ends = cluster_max2(~order_key(hi), lo < INFINITY ? order_key(lo) : 0u, &sh, round);
   Row r;
-  r.m = key_value(~(uint32_t)(top >> 32));
+  r.m = key_value(~ends.x);
   const float t = a.temperature[row];
   if (r.m == -INFINITY) {  // nothing to draw from
     if (me == 0 && tid == 0) {
@@ -351,19 +464,23 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
   u64 last = ~0ull;  // last kept key
   if (cuts[0] || cuts[1]) {
     // bins over what the row spans, where that is less than the weights' reach (high temperatures)
-    const u64 bottom = cluster_join(lo < INFINITY ? (u64)order_key(lo) : 0ull, MAX, &sh, round, nullptr);
-    const float span = fminf(REACH, (r.m - key_value((uint32_t)bottom)) * r.inv_t * 1.001f);
+    const float span = fminf(REACH, (r.m - key_value(ends.y)) * r.inv_t * 1.001f);
     r.bins = span > 1e-6f ? (float)BINS / span : (float)BINS * 1e6f;  // infinities: span = REACH
   }
   for (int cut = 0; cut < 2; ++cut) {
     if (!cuts[cut]) continue;
     float cell = 0.f, fine = 1.f;  // the histogram covers places [cell, cell + BINS / fine)
     u64 target = (u64)r.k, before = 0;
+    bool maxima = cut == 0 && r.k <= THREADS * n_cta / 4;  // 1.15 k keys expected at most
     for (int level = 0;; ++level) {
       for (int i = tid; i < (cut == 0 ? BINS : 3 * BINS); i += THREADS) count[i] = 0;
       if (tid == 0) sh.listed = 0;
       __syncthreads();
-      for (int i = tid; i < n; i += THREADS) {
+      if (maxima) {
+        const float at = r.place(hi);
+        if (at < (float)BINS) atomicAdd(&count[(int)at], 1u);
+      }
+      for (int i = tid; i < n && !maxima; i += THREADS) {
         const float x = xs[i];
         const float at = (r.place(x) - cell) * fine;
         if (at >= 0.f && at < (float)BINS && full_key(x, i0 + i) <= last) {
@@ -398,7 +515,8 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
         const u64 upto = block_scan(f[0] + f[1], sh.warp, &all);
         const u64 cupto = block_scan(c[0] + c[1], sh.warp2, &keys);
         if (level == 0 && cut == 1) target = (u64)max(1ll, (long long)ceil((double)r.p * (double)all));
-        if (tid == 0) sh.verdict = Verdict{target, 0, keys <= CAP ? FINISH : DONE, BINS - 1};  // fewer than k keys have weight
+        // no crossing: fewer than k keys have weight (or fewer than k maxima)
+        if (tid == 0) sh.verdict = Verdict{target, 0, maxima ? KEYS : keys <= CAP ? FINISH : DONE, BINS - 1};
         __syncthreads();
         const u64 want = target - before;
         const u64 b0 = upto - f[0] - f[1], b1 = upto - f[1];
@@ -407,6 +525,7 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
           const u64 through = cupto - (hit == 0 ? c[1] : 0ull);  // keys up to and with the bin
           Verdict v{target, before + (hit == 0 ? b0 : b1), BITS, 2 * tid + hit};
           if (level == 0 && through <= CAP) v.action = FINISH;
+          else if (maxima) v.action = KEYS;
           else if (c[hit] <= CAP) v.action = CUT;
           else if (level == 0) v.action = REFINE;
           sh.verdict = v;
@@ -425,6 +544,12 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
       target = v.target;
       before = v.before;
       if (v.action == DONE) break;
+      if (v.action == KEYS) {
+        maxima = false;
+        before = 0;
+        --level;
+        continue;
+      }
       if (v.action == REFINE) {
         cell = (float)v.bin;
         fine = (float)BINS;
@@ -466,8 +591,23 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
         if (take && base < CAP) st_dsmem(dst + base * 8, key);
       }
       cluster_sync();
+      if (maxima) {  // the maxima did not say how many keys there are
+        const bool over = ld_dsmem_u32(counter) > CAP;
+        cluster_arrive();  // the first CTA outlives this read
+        if (me == 0 || over) cluster_wait();
+        if (over) {
+          maxima = false;
+          before = 0;
+          --level;
+          continue;
+        }
+      }
       if (finish) {
-        if (me == 0) finish_list(a, r, row, min((int)sh.listed, CAP), cut == 1 ? sh.last : 0ull, list, &sh);
+        if (me != 0) return;
+        const int m = min((int)sh.listed, CAP);
+        const u64 all = cut == 1 ? sh.last : 0ull;
+        if (m > 128) finish_list(a, r, row, m, all, list, &sh);
+        else if (tid < 32) finish_short<4>(a, r, row, m, all, list);
         return;
       }
       if (me == 0) {

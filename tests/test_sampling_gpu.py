@@ -122,6 +122,28 @@ def test_ties_take_the_lowest_index():
     assert tok.tolist() == [0] * R
 
 
+@pytest.mark.parametrize("V", [3000, 60000])
+def test_largest_logits_next_to_each_other(V):
+    """Thousands of candidates in the hands of a few threads, and in one place of the histogram."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    R = 6
+    x = torch.randn(R, V, generator=g, device="cuda")
+    x[:, : V // 4] += 9
+    x[3:, V // 2: V // 2 + 1500] = 20.0
+    u = torch.rand(R, generator=g, device="cuda")
+    k = torch.tensor([5, 100, 1500, 3, 1499, 1600], dtype=torch.int32, device="cuda")
+    for p in (None, _f([0.9] * R)):
+        for temp in (1.0, 0.05, 30.0):
+            _check(x, u, _f([temp] * R), k, p, None)
+    _check(x, u, _f([0.5] * R), None, _f([0.02, 0.5, 0.999, 0.02, 0.5, 0.999]), None)
+    # sorted along a thread's own elements: its maximum says little about the others
+    y = torch.sort(x, descending=True).values
+    _check(y, u, _f([1.0] * R), k, None, None)
+    z = torch.full((2, V), -5.0, device="cuda")
+    z[:, ::2048] = torch.arange(0, (V + 2047) // 2048, device="cuda").float() * 0.01
+    _check(z, u[:2], _f([1.0] * 2), k[:2], None, None)
+
+
 @pytest.mark.parametrize("V", [70, 20000])
 def test_degenerate_rows(V):
     inf = float("inf")
