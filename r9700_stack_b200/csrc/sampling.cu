@@ -26,6 +26,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <climits>
+#include <type_traits>
 #include "common.cuh"
 
 namespace r9k {
@@ -229,41 +230,46 @@ R9K_DEVINL float as_logit(float v) { return v != v ? -INFINITY : v; }
 template <>
 R9K_DEVINL float as_logit(__nv_bfloat16 v) { return as_logit(__bfloat162float(v)); }
 
-// The slice's n logits to shared memory as fp32, largest and smallest (finite) on the way: 16-byte
-// loads from the first such boundary on. Returns where they begin (the stores keep the loads' alignment).
+// entries before the first 16-byte boundary of a slice
 template <typename T>
-R9K_DEVINL const float* load_slice(const T* src, int n, float* buf, float& hi, float& lo) {
+R9K_DEVINL int lead(const T* src) { return (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)); }
+
+// Every logit i < n of a slice in global or shared memory, a thread each: four(x, i) for four at a time
+// from the first 16-byte boundary on (four loads in flight), one(x, i) for those around them.
+template <typename T, typename F1, typename F4>
+R9K_DEVINL void scan(const T* src, int n, F1 one, F4 four) {
   constexpr int VEC = 16 / sizeof(T);
-  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)));
-  float* xs = buf + ((4 - (head & 3)) & 3);
-  auto see = [&](float x) {
-    hi = fmaxf(hi, x);
-    if (x > -INFINITY) lo = fminf(lo, x);
-  };
-  const int vecs = (n - head) / VEC;
+  const int head = min(n, lead(src));
+  const int vecs = (n - head) / VEC, rest = head + vecs * VEC;
   const uint4* body = reinterpret_cast<const uint4*>(src + head);
-#pragma unroll 8
-  for (int v = threadIdx.x; v < vecs; v += THREADS) {
-    const uint4 raw = body[v];
+  auto each = [&](uint4 raw, int v) {
     const T* e = reinterpret_cast<const T*>(&raw);
-    float x[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      x[i] = as_logit(e[i]);
-      see(x[i]);
+    for (int i = 0; i < VEC; i += 4) {
+      const float x[4] = {as_logit(e[i]), as_logit(e[i + 1]), as_logit(e[i + 2]), as_logit(e[i + 3])};
+      four(x, head + v * VEC + i);
     }
+  };
+  int v = threadIdx.x;
+  for (; v + 3 * THREADS < vecs; v += 4 * THREADS) {
+    uint4 raw[4];
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4)
-      *reinterpret_cast<float4*>(xs + head + v * VEC + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    for (int j = 0; j < 4; ++j) raw[j] = body[v + j * THREADS];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) each(raw[j], v + j * THREADS);
   }
-  const int rest = head + vecs * VEC;
+  for (; v < vecs; v += THREADS) each(body[v], v);
   for (int i = threadIdx.x; i < head + n - rest; i += THREADS) {
     const int at = i < head ? i : rest + i - head;
-    const float x = as_logit(src[at]);
-    see(x);
-    xs[at] = x;
+    one(as_logit(src[at]), at);
   }
-  return xs;
+}
+template <typename T, typename F>
+R9K_DEVINL void scan(const T* src, int n, F f) {
+  scan(src, n, f, [&](const float (&x)[4], int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f(x[j], i + j);
+  });
 }
 
 // Ascending sort of 32 * E numbers of one warp, number i of lane l at place i * 32 + l.
@@ -404,9 +410,11 @@ R9K_DEVINL void finish_list(const Args& a, const Row& r, int row, int n, u64 all
 }
 }  // namespace sm
 
-template <typename T>
-__global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
+// HELD: the slice is kept in shared memory as fp32; else it is read again (from L2) by each pass
+template <typename T, bool HELD>
+__global__ void __launch_bounds__(sm::THREADS, HELD ? 2 : 3) sample_kernel(const sm::Args a) {
   using namespace sm;
+  using U = std::conditional_t<HELD, float, T>;
   pdl_wait();
   pdl_trigger();
   cluster_arrive();  // every CTA runs before its shared memory is written to (waited for below)
@@ -416,22 +424,46 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
   uint32_t* wlow = count + BINS;
   uint32_t* whigh = wlow + BINS;
   u64* list = reinterpret_cast<u64*>(smem);  // the first CTA's, after the histograms
-  float* buf = reinterpret_cast<float*>(smem + WORK_BYTES);
   const int n_cta = (int)cluster_nctarank(), me = (int)cluster_ctarank();
   const int row = blockIdx.x / n_cta;
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x;
   const int i0 = me * a.slice;
   const int n = max(0, min(a.V - i0, a.slice));
   int round = 0;
+  const float t = a.temperature[row];
+  const float min_p = a.min_p ? a.min_p[row] : 0.f, top_p = a.top_p ? a.top_p[row] : 1.f;
+  const int top_k = a.top_k ? a.top_k[row] : 0;
 
   float hi = -INFINITY, lo = INFINITY;
-  const float* xs = load_slice(reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.ld + i0, n, buf, hi, lo);
+  auto see = [&](float x) {
+    hi = fmaxf(hi, x);
+    if (x > -INFINITY) lo = fminf(lo, x);
+  };
+  const T* src = reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.ld + i0;
+  const U* xs;
+  if constexpr (HELD) {
+    // shifted so that the slice's 16-byte boundaries stay such
+    float* buf = reinterpret_cast<float*>(smem + WORK_BYTES) + ((4 - (lead(src) & 3)) & 3);
+    scan(src, n,
+         [&](float x, int i) {
+           see(x);
+           buf[i] = x;
+         },
+         [&](const float (&x)[4], int i) {
+#pragma unroll
+           for (int j = 0; j < 4; ++j) see(x[j]);
+           *reinterpret_cast<float4*>(buf + i) = make_float4(x[0], x[1], x[2], x[3]);
+         });
+    xs = buf;
+  } else {
+    scan(src, n, [&](float x, int) { see(x); });
+    xs = src;
+  }
   cluster_wait();
   // ~key ascends with the value, a key descends: the largest and the smallest value
   const uint2 ends = cluster_max2(~order_key(hi), lo < INFINITY ? order_key(lo) : 0u, &sh, round);
   Row r;
   r.m = key_value(~ends.x);
-  const float t = a.temperature[row];
   if (r.m == -INFINITY) {  // nothing to draw from
     if (me == 0 && tid == 0) {
       a.tokens[row] = -1;
@@ -441,11 +473,9 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
   }
   if (!(t > 0.f)) {
     uint32_t best = 0;  // ~index
-    for (int i = tid; i < n; i += THREADS)
-      if (xs[i] == r.m) {
-        best = ~(uint32_t)(i0 + i);
-        break;
-      }
+    scan(xs, n, [&](float x, int i) {
+      if (x == r.m) best = max(best, ~(uint32_t)(i0 + i));
+    });
     const u64 first = cluster_join((u64)best, MAX, &sh, round, nullptr);
     if (me == 0 && tid == 0) {
       a.tokens[row] = (int64_t)(uint32_t)~(uint32_t)first;
@@ -454,11 +484,9 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
     return;
   }
   r.inv_t = 1.f / t;
-  r.min_p = a.min_p ? fminf(fmaxf(a.min_p[row], 0.f), 1.f) : 0.f;
-  r.k = a.top_k ? a.top_k[row] : 0;
-  if (r.k < 0 || r.k >= a.V) r.k = 0;
-  r.p = a.top_p ? a.top_p[row] : 1.f;
-  if (!(r.p < 1.f)) r.p = 1.f;
+  r.min_p = fminf(fmaxf(min_p, 0.f), 1.f);
+  r.k = top_k > 0 && top_k < a.V ? top_k : 0;
+  r.p = top_p < 1.f ? top_p : 1.f;
   const bool cuts[2] = {r.k > 0, r.p < 1.f};
 
   u64 last = ~0ull;  // last kept key
@@ -480,22 +508,23 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
         const float at = r.place(hi);
         if (at < (float)BINS) atomicAdd(&count[(int)at], 1u);
       }
-      for (int i = tid; i < n && !maxima; i += THREADS) {
-        const float x = xs[i];
-        const float at = (r.place(x) - cell) * fine;
-        if (at >= 0.f && at < (float)BINS && full_key(x, i0 + i) <= last) {
-          const int bin = (int)at;
-          atomicAdd(&count[bin], 1u);
-          if (cut == 1) {  // 2^31 a weight, 2^16 weights a CTA at most: the halves' sums fit 32 bits
-            const uint32_t w = r.w(x);
-            atomicAdd(&wlow[bin], w & 0xffffu);
-            atomicAdd(&whigh[bin], w >> 16);
+      else
+        scan(xs, n, [&](float x, int i) {
+          const float at = (r.place(x) - cell) * fine;
+          if (at >= 0.f && at < (float)BINS && full_key(x, i0 + i) <= last) {
+            const int bin = (int)at;
+            atomicAdd(&count[bin], 1u);
+            if (cut == 1) {  // 2^31 a weight, fewer than 2^16 weights a CTA: the halves' sums fit 32 bits
+              const uint32_t w = r.w(x);
+              if (w & 0xffffu) atomicAdd(&wlow[bin], w & 0xffffu);
+              if (w >> 16) atomicAdd(&whigh[bin], w >> 16);
+            }
           }
-        }
-      }
+        });
       cluster_sync();
       if (me == 0) {
         u64 c[2] = {0, 0}, f[2] = {0, 0};  // this thread's two bins
+#pragma unroll 4
         for (int i = 0; i < n_cta; ++i) {
           const uint32_t at = mapa_shared(smem_u32(&count[2 * tid]), (uint32_t)i);
           const uint2 v = ld_dsmem_u2(at);
@@ -563,11 +592,11 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
           if (bit < 32 && (1ll << bit) >= 2ll * a.V) continue;  // no index has this bit
           const u64 trial = low | (1ull << bit);
           u64 f = 0;
-          for (int i = tid; i < n; i += THREADS) {
-            const float x = xs[i], at = r.place(x);
+          scan(xs, n, [&](float x, int i) {
+            const float at = r.place(x);
             const u64 key = full_key(x, i0 + i);
             if (at >= from && at < to && key < trial && key <= last) f += cut == 0 ? 1u : r.w(x);
-          }
+          });
           f = cluster_join(f, SUM, &sh, round, nullptr);
           if (before + f < target) low = trial;
         }
@@ -577,19 +606,16 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
       // FINISH: every key up to the bin; CUT: the bin's
       const bool finish = v.action == FINISH;
       const uint32_t counter = mapa_shared(smem_u32(&sh.listed), 0u), dst = mapa_shared(smem_u32(list), 0u);
-      for (int i = tid - lane; i < n; i += THREADS) {
-        const bool in = i + lane < n;
-        const float x = in ? xs[i + lane] : 0.f;
-        const float at = in ? r.place(x) : INFINITY;
-        const u64 key = full_key(x, i0 + i + lane);
-        const bool take = at < to && (finish || at >= from) && key <= last;
-        const uint32_t takers = __ballot_sync(0xffffffffu, take);
-        if (takers == 0) continue;
-        uint32_t base = 0;
-        if (lane == 0) base = add_dsmem(counter, (uint32_t)__popc(takers));
-        base = __shfl_sync(0xffffffffu, base, 0) + (uint32_t)__popc(takers & ((1u << lane) - 1));
-        if (take && base < CAP) st_dsmem(dst + base * 8, key);
-      }
+      scan(xs, n, [&](float x, int i) {
+        const float at = r.place(x);
+        if (at < to && (finish || at >= from)) {
+          const u64 key = full_key(x, i0 + i);
+          if (key <= last) {
+            const uint32_t slot = add_dsmem(counter, 1u);
+            if (slot < CAP) st_dsmem(dst + slot * 8, key);
+          }
+        }
+      });
       cluster_sync();
       if (maxima) {  // the maxima did not say how many keys there are
         const bool over = ld_dsmem_u32(counter) > CAP;
@@ -607,7 +633,8 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
         const int m = min((int)sh.listed, CAP);
         const u64 all = cut == 1 ? sh.last : 0ull;
         if (m > 128) finish_list(a, r, row, m, all, list, &sh);
-        else if (tid < 32) finish_short<4>(a, r, row, m, all, list);
+        else if (tid < 32 && m > 64) finish_short<4>(a, r, row, m, all, list);
+        else if (tid < 32) finish_short<2>(a, r, row, m, all, list);
         return;
       }
       if (me == 0) {
@@ -636,10 +663,9 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
 
   // weights of the kept tokens, a slice a CTA; the draw in index order
   u64 sum = 0;
-  for (int i = tid; i < n; i += THREADS) {
-    const float x = xs[i];
+  scan(xs, n, [&](float x, int i) {
     if (full_key(x, i0 + i) <= last && r.e(x) >= r.min_p) sum += r.w(x);
-  }
+  });
   u64 base;
   const u64 total = cluster_join(sum, SUM, &sh, round, &base);
   const double at = floor((double)a.u[row] * (double)total);
@@ -650,7 +676,7 @@ __global__ void __launch_bounds__(sm::THREADS) sample_kernel(const sm::Args a) {
     const int i = c + tid;
     u64 w = 0;
     if (i < n) {
-      const float x = xs[i];
+      const float x = as_logit(xs[i]);
       if (full_key(x, i0 + i) <= last && r.e(x) >= r.min_p) w = r.w(x);
     }
     u64 all;
@@ -681,26 +707,38 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   if (min_p.has_value()) chk(*min_p, torch::kFloat32, "min_p");
   chk(tokens, torch::kInt64, "tokens");
   chk(logprobs, torch::kFloat32, "logprobs");
-  constexpr int MAX_SLICE = 48 * 1024;  // floats of shared memory
+  constexpr int MAX_SLICE = 48 * 1024;  // floats of shared memory (and fewer than 2^16 weights of a histogram)
   TORCH_CHECK(V <= (int64_t)sm::MAX_CLUSTER * MAX_SLICE, "sample_logits: vocabulary too large");
   if (R == 0) return;
   const at::cuda::CUDAGuard guard(logits.device());
   int C = 1;
   while (C < sm::MAX_CLUSTER && (V + C - 1) / C > 16384) C *= 2;
+  // Slices held in shared memory save the second read, but 16384 logits a CTA leave room for two CTAs an
+  // SM and three quarters of the clusters: while one such wave takes all rows (16 rows x 248320 fp32: 37 us
+  // held in two waves, 28 not). Beyond, fewer and longer slices, read again from L2, three CTAs an SM: 256
+  // rows 271 us held, 250 / 158 / 141 us as 16 / 8 / 4 slices; 64 rows 84 us held, 84 / 61 as 16 / 8.
+  const int64_t sms = device_sm_count();
+  const bool held = R * C <= sms * 3 / 2;
+  if (!held) {
+    C = 1;
+    while (C < sm::MAX_CLUSTER && (R * C < sms * 3 || (V + C - 1) / C > 65532) && (V + C - 1) / C > 4096) C *= 2;
+  }
   TORCH_CHECK(R * C <= INT_MAX, "sample_logits: too many rows");
-  sm::Args a{logits.data_ptr(), logits.stride(0), (int)V, (int)((V + C - 1) / C), u.data_ptr<float>(),
+  sm::Args a{logits.data_ptr(), logits.stride(0), (int)V, (int)((V + C - 1) / C + 3) / 4 * 4, u.data_ptr<float>(),
              temperature.data_ptr<float>(), top_k.has_value() ? top_k->data_ptr<int32_t>() : nullptr,
              top_p.has_value() ? top_p->data_ptr<float>() : nullptr,
              min_p.has_value() ? min_p->data_ptr<float>() : nullptr, tokens.data_ptr<int64_t>(),
              logprobs.data_ptr<float>()};
-  auto kern = logits.dtype() == torch::kFloat32 ? sample_kernel<float> : sample_kernel<__nv_bfloat16>;
-  TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + MAX_SLICE * 4 + 16) == cudaSuccess, "sample_logits: shared memory attribute");
-  TORCH_CHECK(cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess,
-              "sample_logits: cluster attribute");
+  const bool f32 = logits.dtype() == torch::kFloat32;
+  auto kern = held ? (f32 ? sample_kernel<float, true> : sample_kernel<__nv_bfloat16, true>)
+                   : (f32 ? sample_kernel<float, false> : sample_kernel<__nv_bfloat16, false>);
+  TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + (held ? MAX_SLICE * 4 + 16 : 0)) == cudaSuccess &&
+                  cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess,
+              "sample_logits: kernel attributes");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(R * C));
   cfg.blockDim = dim3(sm::THREADS);
-  cfg.dynamicSmemBytes = (size_t)sm::WORK_BYTES + (size_t)a.slice * 4 + 16;
+  cfg.dynamicSmemBytes = (size_t)sm::WORK_BYTES + (held ? (size_t)a.slice * 4 + 16 : 0);
   cfg.stream = at::cuda::getCurrentCUDAStream();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
