@@ -632,7 +632,8 @@ __global__ void __launch_bounds__(sm::THREADS, HELD ? 2 : 3) sample_kernel(const
         if (me != 0) return;
         const int m = min((int)sh.listed, CAP);
         const u64 all = cut == 1 ? sh.last : 0ull;
-        if (m > 128) finish_list(a, r, row, m, all, list, &sh);
+        if (m > 256) finish_list(a, r, row, m, all, list, &sh);
+        else if (tid < 32 && m > 128) finish_short<8>(a, r, row, m, all, list);
         else if (tid < 32 && m > 64) finish_short<4>(a, r, row, m, all, list);
         else if (tid < 32) finish_short<2>(a, r, row, m, all, list);
         return;
@@ -707,24 +708,25 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   if (min_p.has_value()) chk(*min_p, torch::kFloat32, "min_p");
   chk(tokens, torch::kInt64, "tokens");
   chk(logprobs, torch::kFloat32, "logprobs");
-  constexpr int MAX_SLICE = 48 * 1024;  // floats of shared memory (and fewer than 2^16 weights of a histogram)
+  constexpr int MAX_SLICE = 65532;  // a histogram's halves of weights sum to 32 bits
   TORCH_CHECK(V <= (int64_t)sm::MAX_CLUSTER * MAX_SLICE, "sample_logits: vocabulary too large");
   if (R == 0) return;
   const at::cuda::CUDAGuard guard(logits.device());
-  int C = 1;
-  while (C < sm::MAX_CLUSTER && (V + C - 1) / C > 16384) C *= 2;
-  // Slices held in shared memory save the second read, but 16384 logits a CTA leave room for two CTAs an
-  // SM and three quarters of the clusters: while one such wave takes all rows (16 rows x 248320 fp32: 37 us
-  // held in two waves, 28 not). Beyond, fewer and longer slices, read again from L2, three CTAs an SM: 256
-  // rows 271 us held, 250 / 158 / 141 us as 16 / 8 / 4 slices; 64 rows 84 us held, 84 / 61 as 16 / 8.
+  // The most CTAs a row that still let all rows run in one wave (three CTAs an SM, of which clusters of 16
+  // leave a quarter unused), a slice of at least 4096; where no count does, the fewest. Measured, CTAs a row
+  // x 16 / 8 / 4: 256 rows x 248320 fp32, top-k, 250 / 158 / 141 us; 64 rows 84 / 61 / -; 64 rows x 100003,
+  // top-p, - / 66 / 47 us.
   const int64_t sms = device_sm_count();
-  const bool held = R * C <= sms * 3 / 2;
-  if (!held) {
-    C = 1;
-    while (C < sm::MAX_CLUSTER && (R * C < sms * 3 || (V + C - 1) / C > 65532) && (V + C - 1) / C > 4096) C *= 2;
-  }
+  auto slice_of = [&](int c) { return ((V + c - 1) / c + 3) / 4 * 4; };
+  int least = 1;
+  while (slice_of(least) > 65532) least *= 2;
+  int C = sm::MAX_CLUSTER;
+  while (C > least && (slice_of(C) < 4096 || R * C > (C == 16 ? sms * 9 / 4 : sms * 5 / 2))) C /= 2;
+  // Slices held in shared memory are read once, but leave room for two CTAs an SM: while that wave takes
+  // all rows too (64 x 100003, 4 CTAs a row: 45 us held, 47 not; 16 x 248320, 16 CTAs: 37 us held, 28 not).
+  const bool held = slice_of(C) <= 25000 && R * C <= (C == 16 ? sms * 3 / 2 : sms * 7 / 4);
   TORCH_CHECK(R * C <= INT_MAX, "sample_logits: too many rows");
-  sm::Args a{logits.data_ptr(), logits.stride(0), (int)V, (int)((V + C - 1) / C + 3) / 4 * 4, u.data_ptr<float>(),
+  sm::Args a{logits.data_ptr(), logits.stride(0), (int)V, (int)slice_of(C), u.data_ptr<float>(),
              temperature.data_ptr<float>(), top_k.has_value() ? top_k->data_ptr<int32_t>() : nullptr,
              top_p.has_value() ? top_p->data_ptr<float>() : nullptr,
              min_p.has_value() ? min_p->data_ptr<float>() : nullptr, tokens.data_ptr<int64_t>(),
@@ -732,7 +734,7 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   const bool f32 = logits.dtype() == torch::kFloat32;
   auto kern = held ? (f32 ? sample_kernel<float, true> : sample_kernel<__nv_bfloat16, true>)
                    : (f32 ? sample_kernel<float, false> : sample_kernel<__nv_bfloat16, false>);
-  TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + (held ? MAX_SLICE * 4 + 16 : 0)) == cudaSuccess &&
+  TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + (held ? 25000 * 4 + 16 : 0)) == cudaSuccess &&
                   cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess,
               "sample_logits: kernel attributes");
   cudaLaunchConfig_t cfg = {};

@@ -152,6 +152,20 @@ R9K_DEVINL void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   lo = e4m3x2(x - b.x, y - b.y);
 }
 
+// the same for probabilities (0..448): by way of f16, whose conversions are cheaper and whose 2^-12 is far
+// below the lo part's
+R9K_DEVINL void split2p(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 p = __floats2half2_rn(x, y);
+  hi = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(__half2_raw(p), __NV_SATFINITE, __NV_E4M3);
+  const __half2 rest = __hsub2(p, __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)hi, __NV_E4M3)));
+  lo = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(__half2_raw(rest), __NV_SATFINITE, __NV_E4M3);
+}
+R9K_DEVINL float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // 16 bf16 of a row -> 16 bytes hi and lo, scaled
 R9K_DEVINL void split16(const uint4 (&r)[2], float inv, uint4& hi, uint4& lo) {
   const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(r);
@@ -179,14 +193,14 @@ R9K_DEVINL float amax16(const uint4 (&r)[2]) {
 // part's 2^-10 is 2^-16.5 of it or less.
 constexpr float P_SHIFT = 6.5f, P_LAG = 2.25f;
 
-// One value row (key r of a tile, every column half) whose key some of the rows do not see. A NaN code
+// One value row (key r of a tile, column halves [H0, H1)) whose key some of the rows do not see. A NaN code
 // in it would reach those rows too (0 * NaN), so such a row of values is cleared, and the rows that do
 // see its key are marked: they become NaN as a whole. Values of keys that no row sees are stale bytes.
-template <int D>
-R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, int end, int tok0, int ntok, int* poison) {
+template <int H0, int H1, typename P>
+R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, int end, int tok0, int ntok, P* poison) {
   uint32_t nan = 0;
 #pragma unroll
-  for (int h = 0; h < D / 128; ++h)
+  for (int h = H0; h < H1; ++h)
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       const uint4 v = *reinterpret_cast<const uint4*>(tile + h * (KT * 128) + r * 128 + ((c ^ (r & 7)) << 4));
@@ -197,7 +211,7 @@ R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, in
   for (int i = 0; i < ntok; ++i)
     if (key < end && visible(a, key, context(a, tok0 + i))) poison[i] = 1;
 #pragma unroll
-  for (int h = 0; h < D / 128; ++h)
+  for (int h = H0; h < H1; ++h)
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       *reinterpret_cast<uint4*>(tile + h * (KT * 128) + r * 128 + ((c ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
@@ -457,7 +471,7 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
       if (!whole) {
         const int u = unit_v(j);
         w_ok &= __all_sync(0xffffffffu, mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns));
-        clean_value_row<D>(a, smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT, r, key, end, tok0, ntok, poison);
+        clean_value_row<0, C::HALVES>(a, smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT, r, key, end, tok0, ntok, poison);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1)
@@ -607,15 +621,17 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
 // MMA's M side.
 //
 // S = Q K^T [rows x keys] with two S buffers in TMEM, so the next tile's product runs during this
-// tile's softmax; O += P V with V read as it lies (MN-major B operand), O in TMEM. One thread a row
-// reads its scores, keeps the running maximum and sum and writes the probabilities (hi and lo plane).
+// tile's softmax; O += P V with V read as it lies (MN-major B operand), O in TMEM. Two threads a row, in two
+// warpgroups, take 64 keys each: scores from TMEM, the row's running maximum (exchanged through shared
+// memory, one barrier of the two warps a tile), their part of the sum, and the probabilities as two planes.
 // K and V tiles share a ring of slots in the order of use, as above. Few tiles: a cluster of CTAs
 // shares the keys of a tile and joins the partial results through distributed shared memory.
 // ------------------------------------------------------------------------------------------------
 namespace wc {
 using namespace wa;
 constexpr int ROWS = 128;
-constexpr int THREADS = 192;
+constexpr int THREADS = 320;   // TMA, MMA, two softmax warpgroups
+constexpr int SOFT = 256;
 template <int D>
 struct Cfg {
   static constexpr int HALVES = D / 128;
@@ -626,12 +642,12 @@ struct Cfg {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_RING = OFF_Q + 2 * PLANE_Q;
   static constexpr int OFF_P = OFF_RING + SLOTS * UNIT;
-  static constexpr int OFF_ML = OFF_P + 2 * PLANE_P;    // m[ROWS], l[ROWS]
-  static constexpr int OFF_POISON = OFF_ML + 2 * ROWS * 4;  // by token
-  static constexpr int OFF_BAR = OFF_POISON + ROWS * 4;
+  static constexpr int OFF_RED = OFF_P + 2 * PLANE_P;      // maxima [parity][half][ROWS]; at the end l[half][ROWS], m[ROWS]
+  static constexpr int OFF_POISON = OFF_RED + 4 * ROWS * 4;  // bytes by token
+  static constexpr int OFF_BAR = OFF_POISON + ROWS;
   static constexpr int NBAR = 1 + 2 * SLOTS + 6;  // q_full, full[], empty[], s_full[2], s_free[2], p_full, pv_done
   static constexpr int OFF_TMEM = OFF_BAR + NBAR * 8;
-  static constexpr int SMEM = OFF_TMEM + 16 + 1024;
+  static constexpr int SMEM = OFF_TMEM + 16;
   static constexpr int TMEM_COLS = 512;
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(SLOTS * UNIT >= ROWS * D * 4, "the ring holds the partial results");
@@ -646,8 +662,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
   using C = Cfg<D>;
   pdl_wait();
   pdl_trigger();
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_full = bars;
   uint64_t* full = bars + 1;
@@ -657,9 +672,10 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
   uint64_t* p_full = s_free + 2;
   uint64_t* pv_done = p_full + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEM);
-  float* row_m = reinterpret_cast<float*>(smem + C::OFF_ML);
-  float* row_l = row_m + ROWS;
-  int* poison = reinterpret_cast<int*>(smem + C::OFF_POISON);
+  float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
+  float* row_l = red;             // [half][ROWS]
+  float* row_m = red + 2 * ROWS;  // [ROWS]
+  uint8_t* poison = smem + C::OFF_POISON;
 
   const int warp = warp_id(), lane = lane_id();
   const int kvh = blockIdx.y;
@@ -693,6 +709,10 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
     }
   }
   if (seq < 0) return;  // the grid is a bound: the same in the whole cluster
+  if (smem_u32(smem) & 1023) {  // the swizzled tiles need it
+    if (threadIdx.x == 0) report_error(a.status, kErrConfig, 325, (int)smem_u32(smem));
+    return;
+  }
   {
     const int start = a.seq_start[seq], len = a.seq_len[seq];
     if (start < 0 || start > a.T - len) {
@@ -709,16 +729,16 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
   const int nrows = ntok * a.G;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 128);
+    mbar_init(q_full, SOFT);
     for (int s = 0; s < C::SLOTS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_free[s], 128);
+      mbar_init(&s_free[s], SOFT);
     }
-    mbar_init(p_full, 128);
+    mbar_init(p_full, SOFT);
     mbar_init(pv_done, 1);
     fence_mbar_init();
     prefetch_tmap(&tmK);
@@ -796,29 +816,33 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;
+    const int q = warp & 3, half = (warp - 2) >> 2;
     const int r = q * 32 + lane;  // TMEM lane == tile row
     const bool valid = r < nrows;
     const int rt = valid ? r / a.G : 0, rg = r % a.G;
     const int tok = tok0 + rt, head = kvh * a.G + rg;
     const int ctx = valid ? context(a, tok) : 0;
     const int seen = a.window > 0 ? ctx - a.window : 0;  // keys from here on are in the window
-    float sl2 = a.scale_log2;
+    auto pair_bar = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory"); };  // the two warps of these rows
+    float sl2;
     {
       const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + head * D);
       float amax = 0.f;
       if (valid)
+#pragma unroll 4
         for (int c = 0; c < D / 16; ++c) {
           const uint4 raw[2] = {src[2 * c], src[2 * c + 1]};
           amax = fmaxf(amax, amax16(raw));
         }
-      const int e = mx_exponent(amax, 448.f);
-      sl2 *= exp2i(max(e, -126));
-      for (int c = 0; c < D / 16; ++c) {
+      const int e = amax > 0.f ? mx_exponent(amax, 448.f) : 0;
+      sl2 = fmaxf(fabsf(a.scale_log2) * exp2i(max(e, -126)), 1.17549435e-38f);
+      const float inv = copysignf(exp2i(-e), a.scale_log2);  // scores come out with the scale's sign
+#pragma unroll 4
+      for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {
         uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
         if (valid) {
           const uint4 raw[2] = {src[2 * c], src[2 * c + 1]};
-          split16(raw, exp2i(-e), hi, lo);
+          split16(raw, inv, hi, lo);
         }
         uint8_t* dst = smem + C::OFF_Q + (c / 8) * (ROWS * 128) + r * 128 + (((c % 8) ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(dst) = hi;
@@ -830,66 +854,74 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
     float m_ref = -INFINITY, l = 0.f;
     const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
     uint8_t* prow = smem + C::OFF_P + r * 128;
+    constexpr int HK = KT / 2;  // keys of this thread's half
     bool ok = true;
+    // A wait that runs out is told to the other warp of the pair (a NaN in place of the maximum, which
+    // never is one): both leave at the next exchange, so neither is left at their barrier.
     for (int j = 0; j < n; ++j) {
       const int s = j & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns));
-      if (!ok) break;
+      ok &= __all_sync(0xffffffffu, mbar_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns));
       tc_fence_after();
-      float sv[KT];
+      float sv[HK];
 #pragma unroll
-      for (int c = 0; c < KT; c += 16) tmem_ld16(trow + S_COL + s * KT + c, sv + c);
+      for (int c = 0; c < HK; c += 16) tmem_ld16(trow + S_COL + s * KT + half * HK + c, sv + c);
       tmem_ld_wait();
       tc_fence_before();
       mbar_arrive(&s_free[s]);
       const int key0 = sp.key0(j0 + j), end = sp.end(j0 + j);
       const bool whole = key0 + KT <= min(ctx_min, end) && (a.window == 0 || key0 >= ctx_max - a.window);
       float tmax = -INFINITY;
-      if (whole) {
-#pragma unroll
-        for (int c = 0; c < KT; ++c) {
-          sv[c] *= sl2;
-          tmax = fmaxf(tmax, sv[c]);
-        }
-      } else {
+      if (!whole) {
         const int top = min(ctx, end);
 #pragma unroll
-        for (int c = 0; c < KT; ++c) {
-          const int key = key0 + c;
-          sv[c] = key < top && (key >= seen || key < a.sinks) ? sv[c] * sl2 : -INFINITY;
-          tmax = fmaxf(tmax, sv[c]);
+        for (int c = 0; c < HK; ++c) {
+          const int key = key0 + half * HK + c;
+          if (key >= top || (key < seen && key >= a.sinks)) sv[c] = -INFINITY;
         }
-        const int u = unit_v(j);
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns));
-        if (!ok) break;
-        clean_value_row<D>(a, smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT, r, key0 + r, end, tok0, ntok, poison);
+        if (half < C::HALVES) {
+          const int u = unit_v(j);
+          ok &= __all_sync(0xffffffffu, mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns));
+          uint8_t* tile = smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT;
+          if (half == 0) clean_value_row<0, 1>(a, tile, r, key0 + r, end, tok0, ntok, poison);
+          else clean_value_row<C::HALVES - 1, C::HALVES>(a, tile, r, key0 + r, end, tok0, ntok, poison);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < HK; ++c) tmax = fmaxf(tmax, sv[c]);
+      red[(s * 2 + half) * ROWS + r] = ok ? tmax : __int_as_float(0x7fffffff);
+      pair_bar();
+      const float theirs = red[(s * 2 + (half ^ 1)) * ROWS + r];
+      if (!ok || theirs != theirs) {
+        ok = false;
+        break;
       }
       // the P planes and O are free once the PV product of the tile before is done
-      if (j > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns));
-        if (!ok) break;
-        tc_fence_after();
-      }
+      if (j > 0) ok &= __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns));
+      tc_fence_after();
+      tmax = fmaxf(tmax, theirs);
+      if (tmax != -INFINITY) tmax *= sl2;
       const bool need = m_ref != -INFINITY && tmax > m_ref + P_LAG;
       if (__any_sync(0xffffffffu, need)) {
-        const float f = need ? exp2f(m_ref - tmax) : 1.f;
+        const float f = need ? ex2(m_ref - tmax) : 1.f;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          float o[16];
+        for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+          float o[32];
           tmem_ld16(trow + O_COL + c, o);
+          tmem_ld16(trow + O_COL + c + 16, o + 16);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] *= f;
+          for (int i = 0; i < 32; ++i) o[i] *= f;
           tmem_st16(trow + O_COL + c, o);
+          tmem_st16(trow + O_COL + c + 16, o + 16);
         }
         tmem_st_wait();
         l *= f;
       }
       if (need || m_ref == -INFINITY) m_ref = tmax;
       const float off = m_ref == -INFINITY ? 0.f : P_SHIFT - m_ref;  // a row that has seen no key: exp2(-inf) = 0
-      float lsum = 0.f;
+      float ls[2] = {0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KT; c += 16) {
+      for (int c = 0; c < HK; c += 16) {
         uint4 hi, lo;
         uint32_t* ph = reinterpret_cast<uint32_t*>(&hi);
         uint32_t* pl = reinterpret_cast<uint32_t*>(&lo);
@@ -897,36 +929,41 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
         for (int i = 0; i < 4; ++i) {
           float p[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = exp2f(sv[c + 4 * i + k] + off);
-          lsum += (p[0] + p[1]) + (p[2] + p[3]);
+          for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(sv[c + 4 * i + k], sl2, off));
+          ls[0] += p[0] + p[1];
+          ls[1] += p[2] + p[3];
           uint32_t h0, l0, h1, l1;
-          split2(p[0], p[1], h0, l0);
-          split2(p[2], p[3], h1, l1);
+          split2p(p[0], p[1], h0, l0);
+          split2p(p[2], p[3], h1, l1);
           ph[i] = h0 | (h1 << 16);
           pl[i] = l0 | (l1 << 16);
         }
-        uint8_t* dst = prow + (((c / 16) ^ (r & 7)) << 4);
+        uint8_t* dst = prow + (((half * (HK / 16) + c / 16) ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(dst) = hi;
         *reinterpret_cast<uint4*>(dst + C::PLANE_P) = lo;
       }
-      l += lsum;
+      l += ls[0] + ls[1];
       fence_proxy_async();
       tc_fence_before();
       mbar_arrive(p_full);
     }
-    if (ok && n > 0) {
+    if (n > 0 && ok) {
       ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((n - 1) & 1), a.timeout_ns));
       tc_fence_after();
     }
     if (!ok) report_error(a.status, kErrMbarTimeout, 324, r);
     const bool have = n > 0 && ok;
-    asm volatile("bar.sync 1, 128;" ::: "memory");  // poison marks
+    asm volatile("bar.sync 5, 256;" ::: "memory");  // maxima read, poison marks written
     if (valid && poison[rt]) l = __int_as_float(0x7fffffff);
     if (ctx == 0) l = 0.f;  // sees nothing (its scores of whole tiles were not masked)
+    row_l[half * ROWS + r] = have ? l : 0.f;
+    if (half == 0) row_m[r] = have ? m_ref : -INFINITY;
     if (nsplit == 1) {
+      pair_bar();
+      l += row_l[(half ^ 1) * ROWS + r];
       const float inv = have && l != 0.f ? a.v_scale / l : 0.f;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 16) {
         float o[16];
         if (have) {
           tmem_ld16(trow + O_COL + c, o);
@@ -957,7 +994,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
       // stores spread over the banks
       float* part = reinterpret_cast<float*>(smem + C::OFF_RING) + r * D;
 #pragma unroll 1
-      for (int c = 0; c < D && have; c += 16) {
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2) && have; c += 16) {
         float o[16];
         tmem_ld16(trow + O_COL + c, o);
         tmem_ld_wait();
@@ -965,18 +1002,17 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<float4*>(part + (((c / 4 + i) ^ (r & 31)) << 2)) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       }
-      row_m[r] = have ? m_ref : -INFINITY;
-      row_l[r] = have ? l : 0.f;
     }
   }
   tc_fence_before();
   if (nsplit > 1) {
     cluster_sync();
     // rows r = split, split + nsplit, ...: a warp a row, a lane four dims at a time
-    const uint32_t part = smem_u32(smem + C::OFF_RING), ml = smem_u32(row_m);
+    const uint32_t part = smem_u32(smem + C::OFF_RING), ml = smem_u32(row_m), ll = smem_u32(row_l);
     for (int r = split + nsplit * warp; r < nrows; r += nsplit * (THREADS / 32)) {
       const float m_l = lane < nsplit ? ld_dsmem(mapa_shared(ml, (uint32_t)lane) + r * 4) : -INFINITY;
-      const float l_l = lane < nsplit ? ld_dsmem(mapa_shared(ml, (uint32_t)lane) + (ROWS + r) * 4) : 0.f;
+      const uint32_t lat = mapa_shared(ll, (uint32_t)(lane < nsplit ? lane : 0));
+      const float l_l = lane < nsplit ? ld_dsmem(lat + r * 4) + ld_dsmem(lat + (ROWS + r) * 4) : 0.f;
       float M = l_l != 0.f ? m_l : -INFINITY;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
