@@ -122,6 +122,39 @@ R9K_DEVINL void load_tile(const Args& a, const CUtensorMap* map, uint8_t* dst, u
   }
 }
 
+// The MMA warp runs as a whole, so that addresses stay in uniform registers (a lone thread pays dozens of
+// cycles an MMA to move them there), and one elected lane issues: `go` is that lane's predicate.
+R9K_DEVINL void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accum, bool go) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accum), "r"((uint32_t)go)
+      : "memory");
+}
+// A from TMEM: 4 e4m3 numbers of a row in a 32-bit column
+R9K_DEVINL void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accum, bool go) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"((uint32_t)accum), "r"((uint32_t)go)
+      : "memory");
+}
+R9K_DEVINL void commit(uint64_t* bar, bool go) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"((uint32_t)go)
+      : "memory");
+}
+R9K_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t timeout_ns) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, timeout_ns));
+}
+
 // operand descriptor, MN-major 128-byte swizzle (values: head dims contiguous, keys along K)
 R9K_DEVINL uint64_t sdesc_mn(uint32_t saddr) {
   uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
@@ -623,7 +656,10 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
 // S = Q K^T [rows x keys] with two S buffers in TMEM, so the next tile's product runs during this
 // tile's softmax; O += P V with V read as it lies (MN-major B operand), O in TMEM. Two threads a row, in two
 // warpgroups, take 64 keys each: scores from TMEM, the row's running maximum (exchanged through shared
-// memory, one barrier of the two warps a tile), their part of the sum, and the probabilities as two planes.
+// memory, one barrier of the two warps a tile), their part of the sum, and the probabilities as two planes,
+// written over the scores in TMEM: as the A operand of PV they cost no shared memory bandwidth, which is
+// what two products on one K or V tile run into (both planes' MMAs read it). MMAs run in order, so S(j + 2)
+// does not overtake PV(j) on the buffer they share, and only a rescale of O has to wait for PV(j - 1).
 // K and V tiles share a ring of slots in the order of use, as above. Few tiles: a cluster of CTAs
 // shares the keys of a tile and joins the partial results through distributed shared memory.
 // ------------------------------------------------------------------------------------------------
@@ -636,23 +672,21 @@ template <int D>
 struct Cfg {
   static constexpr int HALVES = D / 128;
   static constexpr int UNIT = KT * D;
-  static constexpr int SLOTS = 4;
+  static constexpr int SLOTS = D == 256 ? 5 : 8;
   static constexpr int PLANE_Q = ROWS * D;
-  static constexpr int PLANE_P = ROWS * KT;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_RING = OFF_Q + 2 * PLANE_Q;
-  static constexpr int OFF_P = OFF_RING + SLOTS * UNIT;
-  static constexpr int OFF_RED = OFF_P + 2 * PLANE_P;      // maxima [parity][half][ROWS]; at the end l[half][ROWS], m[ROWS]
+  static constexpr int OFF_RED = OFF_RING + SLOTS * UNIT;  // maxima [parity][half][ROWS]; at the end l[half][ROWS], m[ROWS]
   static constexpr int OFF_POISON = OFF_RED + 4 * ROWS * 4;  // bytes by token
   static constexpr int OFF_BAR = OFF_POISON + ROWS;
-  static constexpr int NBAR = 1 + 2 * SLOTS + 6;  // q_full, full[], empty[], s_full[2], s_free[2], p_full, pv_done
+  static constexpr int NBAR = 1 + 2 * SLOTS + 4;  // q_full, full[], empty[], s_full[2], p_full, pv_done
   static constexpr int OFF_TMEM = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_TMEM + 16;
   static constexpr int TMEM_COLS = 512;
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(SLOTS * UNIT >= ROWS * D * 4, "the ring holds the partial results");
 };
-constexpr int O_COL = 0, S_COL = 256;
+constexpr int O_COL = 0, S_COL = 256;  // two S buffers of 128 columns; P planes at 0 and 32 of them
 }  // namespace wc
 
 template <int D>
@@ -668,8 +702,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
   uint64_t* full = bars + 1;
   uint64_t* empty = full + C::SLOTS;
   uint64_t* s_full = empty + C::SLOTS;
-  uint64_t* s_free = s_full + 2;
-  uint64_t* p_full = s_free + 2;
+  uint64_t* p_full = s_full + 2;
   uint64_t* pv_done = p_full + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEM);
   float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
@@ -734,10 +767,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&s_free[s], SOFT);
-    }
+    for (int s = 0; s < 2; ++s) mbar_init(&s_full[s], 1);
     mbar_init(p_full, SOFT);
     mbar_init(pv_done, 1);
     fence_mbar_init();
@@ -770,49 +800,51 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
       constexpr uint32_t idesc_s = idesc_dense(kFmtE4M3, kFmtE4M3, ROWS, KT);
       constexpr uint32_t idesc_o = idesc_dense(kFmtE4M3, kFmtE4M3, ROWS, D) | (1u << 16);  // B (V) MN-major
-      const uint32_t sq = smem_u32(smem + C::OFF_Q), spp = smem_u32(smem + C::OFF_P);
-      bool ok = mbar_wait(q_full, 0, a.timeout_ns);
-      auto slot = [&](int u) -> uint32_t { return smem_u32(smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT); };
-      auto wait_unit = [&](int u) { return mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns); };
+      const bool go = elect_one();
+      const uint64_t q_desc = sdesc_k_sw128(smem_u32(smem + C::OFF_Q));
+      const uint64_t k_desc = sdesc_k_sw128(smem_u32(smem + C::OFF_RING));
+      const uint64_t v_desc = sdesc_mn(smem_u32(smem + C::OFF_RING));
+      bool ok = warp_wait(q_full, 0, a.timeout_ns);
+      auto wait_unit = [&](int u) { return warp_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns); };
       auto issue_s = [&](int j) -> bool {
-        const int s = j & 1, u = j == 0 ? 0 : 2 * j - 1;
+        const int u = j == 0 ? 0 : 2 * j - 1;
         if (!wait_unit(u)) return false;
-        if (!mbar_wait(&s_free[s], (uint32_t)(((j >> 1) & 1) ^ 1), a.timeout_ns)) return false;
         tc_fence_after();
-        const uint32_t sk = slot(u);
+        const uint64_t kd = k_desc + (uint64_t)((u % C::SLOTS) * (C::UNIT >> 4));
+        const uint32_t d = tbase + S_COL + (j & 1) * KT;
 #pragma unroll
         for (int h = 0; h < C::HALVES; ++h)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
             for (int pl = 0; pl < 2; ++pl)
-              mma_f8f6f4_ss(tbase + S_COL + s * KT, sdesc_k_sw128(sq + pl * C::PLANE_Q + h * (ROWS * 128) + 32 * k),
-                            sdesc_k_sw128(sk + h * (KT * 128) + 32 * k), idesc_s, (h > 0 || k > 0 || pl > 0) ? 1u : 0u);
-        tc_commit(&s_full[s]);
-        tc_commit(&empty[u % C::SLOTS]);
+              mma_ss(d, q_desc + ((pl * C::PLANE_Q + h * (ROWS * 128) + 32 * k) >> 4), kd + ((h * (KT * 128) + 32 * k) >> 4),
+                     idesc_s, h > 0 || k > 0 || pl > 0, go);
+        commit(&s_full[j & 1], go);
+        commit(&empty[u % C::SLOTS], go);
         return true;
       };
       if (ok) ok = issue_s(0);
       for (int j = 0; ok && j < n; ++j) {
         if (j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
         const int u = unit_v(j);
-        if (!mbar_wait(p_full, (uint32_t)(j & 1), a.timeout_ns)) { ok = false; break; }
+        if (!warp_wait(p_full, (uint32_t)(j & 1), a.timeout_ns)) { ok = false; break; }
         if (!wait_unit(u)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t sv = slot(u);
+        const uint64_t vd = v_desc + (uint64_t)((u % C::SLOTS) * (C::UNIT >> 4));
+        const uint32_t p = tbase + S_COL + (j & 1) * KT;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int pl = 0; pl < 2; ++pl)
-            mma_f8f6f4_ss(tbase + O_COL, sdesc_k_sw128(spp + pl * C::PLANE_P + 32 * k), sdesc_mn(sv + k * 4096), idesc_o,
-                          (j > 0 || k > 0 || pl > 0) ? 1u : 0u);
-        tc_commit(pv_done);
-        tc_commit(&empty[u % C::SLOTS]);
+            mma_ts(tbase + O_COL, p + pl * 32 + 8 * k, vd + (k * 4096 >> 4), idesc_o, j > 0 || k > 0 || pl > 0, go);
+        commit(pv_done, go);
+        commit(&empty[u % C::SLOTS], go);
       }
-      if (!ok) report_error(a.status, kErrMbarTimeout, 323, 0);
+      if (!ok && lane == 0) report_error(a.status, kErrMbarTimeout, 323, 0);
     }
     __syncwarp();
   } else {
@@ -853,21 +885,18 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
     }
     float m_ref = -INFINITY, l = 0.f;
     const uint32_t trow = tbase + ((uint32_t)(q * 32) << 16);
-    uint8_t* prow = smem + C::OFF_P + r * 128;
     constexpr int HK = KT / 2;  // keys of this thread's half
     bool ok = true;
     // A wait that runs out is told to the other warp of the pair (a NaN in place of the maximum, which
     // never is one): both leave at the next exchange, so neither is left at their barrier.
     for (int j = 0; j < n; ++j) {
       const int s = j & 1;
-      ok &= __all_sync(0xffffffffu, mbar_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns));
+      ok &= warp_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns);
       tc_fence_after();
       float sv[HK];
 #pragma unroll
       for (int c = 0; c < HK; c += 16) tmem_ld16(trow + S_COL + s * KT + half * HK + c, sv + c);
       tmem_ld_wait();
-      tc_fence_before();
-      mbar_arrive(&s_free[s]);
       const int key0 = sp.key0(j0 + j), end = sp.end(j0 + j);
       const bool whole = key0 + KT <= min(ctx_min, end) && (a.window == 0 || key0 >= ctx_max - a.window);
       float tmax = -INFINITY;
@@ -880,7 +909,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
         }
         if (half < C::HALVES) {
           const int u = unit_v(j);
-          ok &= __all_sync(0xffffffffu, mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns));
+          ok &= warp_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns);
           uint8_t* tile = smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT;
           if (half == 0) clean_value_row<0, 1>(a, tile, r, key0 + r, end, tok0, ntok, poison);
           else clean_value_row<C::HALVES - 1, C::HALVES>(a, tile, r, key0 + r, end, tok0, ntok, poison);
@@ -895,14 +924,36 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
         ok = false;
         break;
       }
-      // the P planes and O are free once the PV product of the tile before is done
-      if (j > 0) ok &= __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns));
-      tc_fence_after();
       tmax = fmaxf(tmax, theirs);
       if (tmax != -INFINITY) tmax *= sl2;
       const bool need = m_ref != -INFINITY && tmax > m_ref + P_LAG;
+      const float f = need ? ex2(m_ref - tmax) : 1.f;
+      if (need || m_ref == -INFINITY) m_ref = tmax;
+      const float off = m_ref == -INFINITY ? 0.f : P_SHIFT - m_ref;  // a row that has seen no key: exp2(-inf) = 0
+      float ls[2] = {0.f, 0.f};
+      float ph[HK / 4], pl[HK / 4];  // four e4m3 numbers each
+#pragma unroll
+      for (int c = 0; c < HK; c += 4) {
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(sv[c + k], sl2, off));
+        ls[0] += p[0] + p[1];
+        ls[1] += p[2] + p[3];
+        uint32_t h0, l0, h1, l1;
+        split2p(p[0], p[1], h0, l0);
+        split2p(p[2], p[3], h1, l1);
+        ph[c / 4] = __uint_as_float(h0 | (h1 << 16));
+        pl[c / 4] = __uint_as_float(l0 | (l1 << 16));
+      }
+      l = l * f + (ls[0] + ls[1]);
+      // both threads of the row have read their scores (the exchange came after)
+      const uint32_t pcol = trow + S_COL + s * KT + half * (HK / 4);
+      tmem_st16(pcol, ph);
+      tmem_st16(pcol + 32, pl);
       if (__any_sync(0xffffffffu, need)) {
-        const float f = need ? ex2(m_ref - tmax) : 1.f;
+        // (S(j) came after PV(j - 2): this product is the only one that may not be done)
+        if (j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
+        tc_fence_after();
 #pragma unroll 1
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
           float o[32];
@@ -914,43 +965,16 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
           tmem_st16(trow + O_COL + c, o);
           tmem_st16(trow + O_COL + c + 16, o + 16);
         }
-        tmem_st_wait();
-        l *= f;
       }
-      if (need || m_ref == -INFINITY) m_ref = tmax;
-      const float off = m_ref == -INFINITY ? 0.f : P_SHIFT - m_ref;  // a row that has seen no key: exp2(-inf) = 0
-      float ls[2] = {0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < HK; c += 16) {
-        uint4 hi, lo;
-        uint32_t* ph = reinterpret_cast<uint32_t*>(&hi);
-        uint32_t* pl = reinterpret_cast<uint32_t*>(&lo);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float p[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(sv[c + 4 * i + k], sl2, off));
-          ls[0] += p[0] + p[1];
-          ls[1] += p[2] + p[3];
-          uint32_t h0, l0, h1, l1;
-          split2p(p[0], p[1], h0, l0);
-          split2p(p[2], p[3], h1, l1);
-          ph[i] = h0 | (h1 << 16);
-          pl[i] = l0 | (l1 << 16);
-        }
-        uint8_t* dst = prow + (((half * (HK / 16) + c / 16) ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = hi;
-        *reinterpret_cast<uint4*>(dst + C::PLANE_P) = lo;
-      }
-      l += ls[0] + ls[1];
-      fence_proxy_async();
+      tmem_st_wait();
       tc_fence_before();
       mbar_arrive(p_full);
     }
-    if (n > 0 && ok) {
-      ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (uint32_t)((n - 1) & 1), a.timeout_ns));
-      tc_fence_after();
-    }
+    // S(n - 1) came after PV(n - 3), so up to two products are still to come: one phase at a time, since a
+    // parity does not tell the last from the one before the last but one
+    if (n > 1 && ok) ok = warp_wait(pv_done, (uint32_t)((n - 2) & 1), a.timeout_ns);
+    if (n > 0 && ok) ok = warp_wait(pv_done, (uint32_t)((n - 1) & 1), a.timeout_ns);
+    tc_fence_after();
     if (!ok) report_error(a.status, kErrMbarTimeout, 324, r);
     const bool have = n > 0 && ok;
     asm volatile("bar.sync 5, 256;" ::: "memory");  // maxima read, poison marks written
