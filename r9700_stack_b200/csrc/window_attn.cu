@@ -45,24 +45,29 @@ struct Args {
   uint64_t timeout_ns;
 };
 
-// The visible keys of a group of rows as tiles of KT keys: first the sinks [0, sk), then the window
-// [base, lim) from a page boundary on.
+// The keys that a group of rows can see, as a list of pages: those of the sinks first, then the window's
+// from a page boundary on. A tile is two neighbours of the list.
+constexpr int NO_KEY = INT_MAX / 2;
 struct Span {
-  int base, lim, sk, n_sink, n;
-  R9K_DEVINL int key0(int j) const { return j < n_sink ? j * KT : base + (j - n_sink) * KT; }
-  R9K_DEVINL int end(int j) const { return j < n_sink ? sk : lim; }
+  int base, n_sink, pages, n;  // first window page, pages of the sinks, pages, tiles
+  R9K_DEVINL int key(int i) const {  // first key of page i of the list; NO_KEY past its end
+    return i < n_sink ? i * PAGE : i < pages ? (base + i - n_sink) * PAGE : NO_KEY;
+  }
 };
 
 // ctx_min, ctx_max: smallest and largest context of the rows that see anything (0, 0: none does)
 R9K_DEVINL Span make_span(const Args& a, int ctx_min, int ctx_max) {
   Span s;
-  const int lo = a.window > 0 ? max(0, ctx_min - a.window) : 0;
-  s.base = lo / PAGE * PAGE;
-  s.lim = ctx_max;
-  s.sk = min(a.sinks, s.base);
-  s.n_sink = (s.sk + KT - 1) / KT;
-  s.n = s.n_sink + (ctx_max > s.base ? (ctx_max - s.base + KT - 1) / KT : 0);
+  s.base = (a.window > 0 ? max(0, ctx_min - a.window) : 0) / PAGE;
+  s.n_sink = min((a.sinks + PAGE - 1) / PAGE, s.base);
+  s.pages = s.n_sink + max(0, (ctx_max + PAGE - 1) / PAGE - s.base);
+  s.n = (s.pages + 1) / 2;
   return s;
+}
+
+// whether every row (contexts in [ctx_min, ctx_max]) sees the whole page at key
+R9K_DEVINL bool whole_page(const Args& a, int key, int ctx_min, int ctx_max) {
+  return key + PAGE <= ctx_min && (a.window == 0 || key >= ctx_max - a.window || key + PAGE <= a.sinks);
 }
 
 R9K_DEVINL bool visible(const Args& a, int key, int ctx) {
@@ -105,20 +110,36 @@ R9K_DEVINL int page_of(const Args& a, int seq, int key) {
   return p;
 }
 
-// K or V tile j -> shared memory: two pages, D / 128 column halves, 128-byte swizzled rows. A page past
-// the tile's end is not looked up (its rows are masked): page 0 stands in for it.
+// The loading warp's view of the page list: 32 page numbers at a time, a lane each, so that the table's
+// latency is paid once in 16 tiles and not once a tile.
+struct Pages {
+  int first = -1, mine = 0;  // list index of lane 0's page
+  R9K_DEVINL int get(const Args& a, const Span& sp, int seq, int i, int origin) {
+    const int f = origin + (i - origin) / 32 * 32;
+    if (f != first) {
+      first = f;
+      const int key = sp.key(f + (int)lane_id());
+      mine = key != NO_KEY ? page_of(a, seq, key) : 0;  // page 0 stands in past the list's end (masked)
+    }
+    return __shfl_sync(0xffffffffu, mine, i - f);
+  }
+};
+
+// K or V tile j -> shared memory: two pages, D / 128 column halves, 128-byte swizzled rows. A whole warp;
+// `go` is true in the lane that issues.
 template <int D>
-R9K_DEVINL void load_tile(const Args& a, const CUtensorMap* map, uint8_t* dst, uint64_t* bar, const Span& sp, int j, int seq,
-                          int kvh) {
-  const int key0 = sp.key0(j), end = sp.end(j);
-  mbar_arrive_expect_tx(bar, KT * D);
+R9K_DEVINL void load_tile(const Args& a, const CUtensorMap* map, uint8_t* dst, uint64_t* bar, const Span& sp, Pages& pages, int j,
+                          int origin, int seq, int kvh, bool go) {
+  int page[2];
 #pragma unroll
-  for (int p = 0; p < KT / PAGE; ++p) {
-    const int key = key0 + p * PAGE;
-    const int page = key < end ? page_of(a, seq, key) : 0;
+  for (int p = 0; p < 2; ++p) page[p] = pages.get(a, sp, seq, 2 * j + p, 2 * origin);
+  if (go) {
+    mbar_arrive_expect_tx(bar, KT * D);
 #pragma unroll
-    for (int h = 0; h < D / 128; ++h)
-      tma_load_2d(dst + h * (KT * 128) + p * (PAGE * 128), map, bar, h * 128, (page * a.Hkv + kvh) * PAGE);
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int h = 0; h < D / 128; ++h)
+        tma_load_2d(dst + h * (KT * 128) + p * (PAGE * 128), map, bar, h * 128, (page[p] * a.Hkv + kvh) * PAGE);
   }
 }
 
@@ -230,7 +251,7 @@ constexpr float P_SHIFT = 6.5f, P_LAG = 2.25f;
 // in it would reach those rows too (0 * NaN), so such a row of values is cleared, and the rows that do
 // see its key are marked: they become NaN as a whole. Values of keys that no row sees are stale bytes.
 template <int H0, int H1, typename P>
-R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, int end, int tok0, int ntok, P* poison) {
+R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, int tok0, int ntok, P* poison) {
   uint32_t nan = 0;
 #pragma unroll
   for (int h = H0; h < H1; ++h)
@@ -242,7 +263,7 @@ R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, in
     }
   if ((nan & 0x80808080u) == 0) return;
   for (int i = 0; i < ntok; ++i)
-    if (key < end && visible(a, key, context(a, tok0 + i))) poison[i] = 1;
+    if (visible(a, key, context(a, tok0 + i))) poison[i] = 1;
 #pragma unroll
   for (int h = H0; h < H1; ++h)
 #pragma unroll
@@ -264,27 +285,29 @@ R9K_DEVINL void clean_value_row(const Args& a, uint8_t* tile, int r, int key, in
 // ------------------------------------------------------------------------------------------------
 namespace wd {
 using namespace wa;
-constexpr int N = 16;          // query rows of a tile
+constexpr int ROWS = 16;  // most query rows
 constexpr int THREADS = 192;
-template <int D>
+template <int D, int NC>
 struct Cfg {
+  static constexpr int N = 2 * NC;  // columns: the rows' hi planes, then their lo planes
   static constexpr int HALVES = D / 128;
   static constexpr int UNIT = KT * D;                 // one K or V tile
   static constexpr int SLOTS = D == 256 ? 3 : 6;      // two CTAs on an SM
-  static constexpr int PLANE_Q = HALVES * N * 128;    // hi or lo plane of Q: a swizzled tile a half
-  static constexpr int PLANE_P = N * 128;
+  static constexpr int Q_BYTES = HALVES * N * 128;    // a swizzled tile a column half
+  static constexpr int P_BYTES = N * 128;
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_RING = OFF_Q + 2 * PLANE_Q;
-  static constexpr int OFF_P = OFF_RING + SLOTS * UNIT;  // [parity][hi, lo]
-  static constexpr int OFF_RED = OFF_P + 4 * PLANE_P;    // float [parity][max, sum][4 warps][N]
-  static constexpr int OFF_COL = OFF_RED + 2 * 2 * 4 * N * 4;  // scale[N], ctx[N], poison[N], m[N], l[N]
-  static constexpr int OFF_BAR = OFF_COL + 5 * N * 4;
+  static constexpr int OFF_RING = OFF_Q + Q_BYTES;
+  static constexpr int OFF_P = OFF_RING + SLOTS * UNIT;     // [parity]
+  static constexpr int OFF_RED = OFF_P + 2 * P_BYTES;       // float maxima [parity][NC][4 warps]; at the end sums
+  static constexpr int OFF_COL = OFF_RED + 2 * 4 * NC * 4;  // scale, ctx, poison (by token), m, l [ROWS]
+  static constexpr int OFF_W = OFF_COL + 5 * ROWS * 4;      // weights of the cluster's partial results [ROWS][8]
+  static constexpr int OFF_BAR = OFF_W + ROWS * 8 * 4;
   static constexpr int NBAR = 1 + 2 * SLOTS + 8;  // q_full, full[], empty[], s_full[2], s_free[2], p_full[2], pv_done[2]
   static constexpr int OFF_TMEM = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_TMEM + 16 + 1024;
+  static constexpr int TMEM_COLS = 4 * N;
+  static constexpr int S_COL = 0, O_COL = 2 * N;  // two S buffers, O^T halves
 };
-constexpr int TMEM_COLS = 64;
-constexpr int S_COL = 0, O_COL = 32;  // S buffers [0, 32), O^T halves [32, 64)
 }  // namespace wd
 
 R9K_DEVINL void wd_bar() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -293,7 +316,8 @@ template <int D, int NC>
 __global__ void __launch_bounds__(wd::THREADS, 2)
     window_attn_dec_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const wa::Args a) {
   using namespace wd;
-  using C = Cfg<D>;
+  using C = Cfg<D, NC>;
+  constexpr int N = C::N, S_COL = C::S_COL, O_COL = C::O_COL;
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
@@ -309,11 +333,11 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEM);
   float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
   float* col_scale = reinterpret_cast<float*>(smem + C::OFF_COL);
-  int* col_ctx = reinterpret_cast<int*>(col_scale + N);
-  int* poison = col_ctx + N;  // by token
-  float* col_m = reinterpret_cast<float*>(poison + N);
-  float* col_l = col_m + N;
-  __shared__ int s_fail;
+  int* col_ctx = reinterpret_cast<int*>(col_scale + ROWS);
+  int* poison = col_ctx + ROWS;  // by token
+  float* col_m = reinterpret_cast<float*>(poison + ROWS);
+  float* col_l = col_m + ROWS;
+  float* weight = reinterpret_cast<float*>(smem + C::OFF_W);
 
   const int warp = warp_id(), lane = lane_id();
   const int seq = blockIdx.x, kvh = blockIdx.y;
@@ -333,7 +357,6 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
   const int NQ = ntok * a.G;  // <= NC
 
   if (threadIdx.x == 0) {
-    s_fail = 0;
     mbar_init(q_full, 128);
     for (int s = 0; s < C::SLOTS; ++s) {
       mbar_init(&full[s], 1);
@@ -349,9 +372,9 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
   }
-  if (threadIdx.x < N) poison[threadIdx.x] = 0;
+  if (threadIdx.x < ROWS) poison[threadIdx.x] = 0;
   if (warp == 1) {
-    tmem_alloc(tmem_holder, TMEM_COLS);
+    tmem_alloc(tmem_holder, C::TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -362,78 +385,76 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
   auto unit_v = [&](int j) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
 
   if (warp == 0) {
-    if (lane == 0) {
-      for (int u = 0; u < 2 * n; ++u) {
+    const bool go = elect_one();
+    Pages pages;
+    for (int u = 0; u < 2 * n; ++u) {
         const bool is_k = u == 0 || ((u & 1) && u < 2 * n - 1);
         const int j = is_k ? (u + 1) / 2 : (u == 2 * n - 1 ? n - 1 : u / 2 - 1);
         const int s = u % C::SLOTS;
-        if (!mbar_wait(&empty[s], (uint32_t)(((u / C::SLOTS) & 1) ^ 1), a.timeout_ns)) {
-          report_error(a.status, kErrMbarTimeout, 311, u);
+        if (!warp_wait(&empty[s], (uint32_t)(((u / C::SLOTS) & 1) ^ 1), a.timeout_ns)) {
+          if (go) report_error(a.status, kErrMbarTimeout, 311, u);
           break;
         }
-        load_tile<D>(a, is_k ? &tmK : &tmV, smem + C::OFF_RING + s * C::UNIT, &full[s], sp, j0 + j, seq, kvh);
+        load_tile<D>(a, is_k ? &tmK : &tmV, smem + C::OFF_RING + s * C::UNIT, &full[s], sp, pages, j0 + j, j0, seq, kvh, go);
       }
-    }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
       constexpr uint32_t idesc_s = idesc_dense(kFmtE4M3, kFmtE4M3, KT, N);
       constexpr uint32_t idesc_o = idesc_dense(kFmtE4M3, kFmtE4M3, 128, N) | (1u << 15);  // A (V^T) MN-major
-      const uint32_t sq = smem_u32(smem + C::OFF_Q);
-      bool ok = mbar_wait(q_full, 0, a.timeout_ns);
-      auto slot = [&](int u) -> uint32_t { return smem_u32(smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT); };
-      auto wait_unit = [&](int u) { return mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns); };
+      const bool go = elect_one();
+      const uint64_t q_desc = sdesc_k_sw128(smem_u32(smem + C::OFF_Q));
+      const uint64_t k_desc = sdesc_k_sw128(smem_u32(smem + C::OFF_RING));
+      const uint64_t v_desc = sdesc_mn(smem_u32(smem + C::OFF_RING));
+      const uint64_t p_desc = sdesc_k_sw128(smem_u32(smem + C::OFF_P));
+      bool ok = warp_wait(q_full, 0, a.timeout_ns);
+      auto wait_unit = [&](int u) { return warp_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns); };
       auto issue_s = [&](int j) -> bool {
         const int s = j & 1, u = j == 0 ? 0 : 2 * j - 1;
         if (!wait_unit(u)) return false;
-        if (!mbar_wait(&s_free[s], (uint32_t)(((j >> 1) & 1) ^ 1), a.timeout_ns)) return false;
+        if (!warp_wait(&s_free[s], (uint32_t)(((j >> 1) & 1) ^ 1), a.timeout_ns)) return false;
         tc_fence_after();
-        const uint32_t sk = slot(u);
+        const uint64_t kd = k_desc + (uint64_t)((u % C::SLOTS) * (C::UNIT >> 4));
 #pragma unroll
         for (int h = 0; h < C::HALVES; ++h)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int pl = 0; pl < 2; ++pl)
-              mma_f8f6f4_ss(tbase + S_COL + s * N, sdesc_k_sw128(sk + h * (KT * 128) + 32 * k),
-                            sdesc_k_sw128(sq + pl * C::PLANE_Q + h * (N * 128) + 32 * k), idesc_s,
-                            (h > 0 || k > 0 || pl > 0) ? 1u : 0u);
-        tc_commit(&s_full[s]);
-        tc_commit(&empty[u % C::SLOTS]);
+            mma_ss(tbase + S_COL + s * N, kd + ((h * (KT * 128) + 32 * k) >> 4), q_desc + ((h * (N * 128) + 32 * k) >> 4),
+                   idesc_s, h > 0 || k > 0, go);
+        commit(&s_full[s], go);
+        commit(&empty[u % C::SLOTS], go);
         return true;
       };
       if (ok) ok = issue_s(0);
       for (int j = 0; ok && j < n; ++j) {
         if (j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
         const int pb = j & 1, u = unit_v(j);
-        if (!mbar_wait(&p_full[pb], (uint32_t)((j >> 1) & 1), a.timeout_ns)) { ok = false; break; }
+        if (!warp_wait(&p_full[pb], (uint32_t)((j >> 1) & 1), a.timeout_ns)) { ok = false; break; }
         if (!wait_unit(u)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t sv = slot(u), spp = smem_u32(smem + C::OFF_P + pb * 2 * C::PLANE_P);
+        const uint64_t vd = v_desc + (uint64_t)((u % C::SLOTS) * (C::UNIT >> 4));
+        const uint64_t pd = p_desc + (uint64_t)(pb * C::P_BYTES >> 4);
 #pragma unroll
         for (int h = 0; h < C::HALVES; ++h)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int pl = 0; pl < 2; ++pl)
-              mma_f8f6f4_ss(tbase + O_COL + h * N, sdesc_mn(sv + h * (KT * 128) + k * 4096),
-                            sdesc_k_sw128(spp + pl * C::PLANE_P + 32 * k), idesc_o, (j > 0 || k > 0 || pl > 0) ? 1u : 0u);
-        tc_commit(&pv_done[pb]);
-        tc_commit(&empty[u % C::SLOTS]);
+            mma_ss(tbase + O_COL + h * N, vd + ((h * (KT * 128) + k * 4096) >> 4), pd + (32 * k >> 4), idesc_o, j > 0 || k > 0,
+                   go);
+        commit(&pv_done[pb], go);
+        commit(&empty[u % C::SLOTS], go);
       }
-      if (!ok) report_error(a.status, kErrMbarTimeout, 312, 0);
+      if (!ok && lane == 0) report_error(a.status, kErrMbarTimeout, 312, 0);
     }
     __syncwarp();
   } else {
     const int q = warp & 3;
     const int r = q * 32 + lane;      // TMEM lane: key of the tile, then dim of the output
     const int tr = threadIdx.x - 64;  // 0..127
-    // rows of P past NQ stay zero; eight threads a query row
-    for (int i = tr; i < 4 * C::PLANE_P / 16; i += 128) reinterpret_cast<uint4*>(smem + C::OFF_P)[i] = make_uint4(0, 0, 0, 0);
+    // columns past NQ: a zero query and context 0, so every key is masked; eight threads a query row
     {
       const int row = tr >> 3, part = tr & 7;
       const bool valid = row < NQ;
-      const int tok = tok0 + row / a.G, head = kvh * a.G + row % a.G;
+      const int tok = tok0 + (valid ? row / a.G : 0), head = kvh * a.G + row % a.G;
       constexpr int CH = D / 128;  // 16-element chunks a thread
       uint4 raw[CH][2];
       float amax = 0.f;
@@ -452,200 +473,240 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       const int e = mx_exponent(amax, 448.f);
+      if (row < NC) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        uint4 hi, lo;
-        split16(raw[c], exp2i(-e), hi, lo);
-        uint8_t* dst = smem + C::OFF_Q + c * (N * 128) + row * 128 + ((part ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = hi;
-        *reinterpret_cast<uint4*>(dst + C::PLANE_Q) = lo;
-      }
-      if (part == 0) {
-        col_scale[row] = a.scale_log2 * exp2i(max(e, -126));
-        col_ctx[row] = valid ? context(a, tok) : 0;
+        for (int c = 0; c < CH; ++c) {
+          uint4 hi, lo;
+          split16(raw[c], exp2i(-e), hi, lo);
+          uint8_t* dst = smem + C::OFF_Q + c * (N * 128) + row * 128 + ((part ^ (row & 7)) << 4);  // NC % 8 == 0: lo alike
+          *reinterpret_cast<uint4*>(dst) = hi;
+          *reinterpret_cast<uint4*>(dst + NC * 128) = lo;
+        }
+        if (part == 0) {
+          col_scale[row] = a.scale_log2 * exp2i(max(e, -126));
+          col_ctx[row] = valid ? context(a, tok) : 0;
+        }
       }
       fence_proxy_async();
       mbar_arrive(q_full);
     }
     wd_bar();
     float mref[NC], lsum[NC], csc[NC];
-    int cctx[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       mref[c] = -INFINITY;
       lsum[c] = 0.f;
       csc[c] = col_scale[c];
-      cctx[c] = col_ctx[c];
     }
-    // a wait that runs out only raises s_fail: the loop is left at the end of a tile, by all together
+    // A wait that runs out is told to the other warps (a NaN in place of a maximum, which never is one):
+    // all four leave at the same exchange, so none is left at their barrier.
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int s = j & 1, pb = j & 1;
-      bool w_ok = __all_sync(0xffffffffu, mbar_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns));
+      ok &= warp_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns);
       tc_fence_after();
-      float sv[16];
-      tmem_ld16(tbase + ((uint32_t)(q * 32) << 16) + S_COL + s * N, sv);
+      float sv[N];
+#pragma unroll
+      for (int c = 0; c < N; c += 16) tmem_ld16(tbase + ((uint32_t)(q * 32) << 16) + S_COL + s * N + c, sv + c);
       tmem_ld_wait();
       tc_fence_before();
       mbar_arrive(&s_free[s]);
-      const int key0 = sp.key0(j0 + j), end = sp.end(j0 + j);
-      const int key = key0 + r;
-      // every row sees the whole tile: no key of it has to be masked
-      const bool whole = key0 + KT <= min(ctx_min, end) && (a.window == 0 || key0 >= ctx_max - a.window);
-      float* rmax = red + pb * 8 * N;
-      float* rsum = rmax + 4 * N;
+      const int key0 = sp.key(2 * (j0 + j) + (q >> 1));  // of this warp's page
+      const int key = key0 + (r & (PAGE - 1));
+      const bool whole = whole_page(a, key0, ctx_min, ctx_max);
+      float* rmax = red + pb * 4 * NC;
       float mx[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const bool vis = key < end && visible(a, key, cctx[c]);
-        sv[c] = vis ? sv[c] * csc[c] : -INFINITY;
-        mx[c] = sv[c];
+        sv[c] = (sv[c] + sv[NC + c]) * csc[c];
+        if (!whole && !visible(a, key, col_ctx[c])) sv[c] = -INFINITY;
+        mx[c] = fmaxf(sv[c], -INFINITY);  // not a NaN
       }
+      // the warp's maxima: each step halves the columns a lane answers for, so NC / 2 + NC / 4 ... exchanges
+      // do where a butterfly of every column takes 5 NC
+#pragma unroll
+      for (int w = NC / 2, o = 16; w > 0; w >>= 1, o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c)
+          if (c < w) {
+            const float keep = up ? mx[c + w] : mx[c], give = up ? mx[c] : mx[c + w];
+            mx[c] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
+          }
+      }
+#pragma unroll
+      for (int o = 16 / NC; o > 0; o >>= 1) mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+      // lane's column: its top bits, the highest first
+      if ((lane & (32 / NC - 1)) == 0) rmax[(lane / (32 / NC)) * 4 + q] = ok ? mx[0] : __int_as_float(0x7fffffff);
       if (!whole) {
         const int u = unit_v(j);
-        w_ok &= __all_sync(0xffffffffu, mbar_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns));
-        clean_value_row<0, C::HALVES>(a, smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT, r, key, end, tok0, ntok, poison);
+        ok &= warp_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns);
+        clean_value_row<0, C::HALVES>(a, smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT, r, key, tok0, ntok, poison);
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], o));
-      if (lane == 0) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) rmax[q * N + c] = mx[c];
-      }
+      // P buffer pb is free once the PV of tile j - 2 is done
+      if (j >= 2) ok &= warp_wait(&pv_done[pb], (uint32_t)(((j - 2) >> 1) & 1), a.timeout_ns);
       wd_bar();
-      float fac[16];
-      bool any = false;
-#pragma unroll
-      for (int c = 0; c < 16; ++c) fac[c] = 1.f;
+      float t[NC];
+      bool any = false, fail = false;  // by what was exchanged alone; a later failure is told with the next tile
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const float t = fmaxf(fmaxf(rmax[c], rmax[N + c]), fmaxf(rmax[2 * N + c], rmax[3 * N + c]));
-        const bool first = mref[c] == -INFINITY;
-        if (!first && t > mref[c] + P_LAG) {
-          fac[c] = exp2f(mref[c] - t);
-          any = true;
-          mref[c] = t;
-        } else if (first) {
-          mref[c] = t;
+        const float4 m4 = *reinterpret_cast<const float4*>(rmax + c * 4);
+        if (c == 0) fail = m4.x != m4.x || m4.y != m4.y || m4.z != m4.z || m4.w != m4.w;
+        t[c] = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+        any |= t[c] > mref[c] + P_LAG;  // the first key seen among them
+      }
+      if (fail) {  // known to all: rmax of this tile is not written again before they have read it
+        ok = false;
+        break;
+      }
+      if (any) {
+        float fac[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const bool need = t[c] > mref[c] + P_LAG;
+          fac[c] = need ? ex2(mref[c] - t[c]) : 1.f;  // 0 for the first
+          if (need) mref[c] = t[c];
+          lsum[c] *= fac[c];
+        }
+        if (j >= 1) {
+          // O is complete before it is rescaled
+          ok &= warp_wait(&pv_done[(j - 1) & 1], (uint32_t)(((j - 1) >> 1) & 1), a.timeout_ns);
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+            for (int c0 = 0; c0 < N; c0 += 16) {
+              const uint32_t orow = tbase + ((uint32_t)(q * 32) << 16) + O_COL + h * N + c0;
+              float o[16];
+              tmem_ld16(orow, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] *= fac[(c0 + i) % NC];
+              tmem_st16(orow, o);
+            }
+          tmem_st_wait();
         }
       }
-      // P buffer pb is free once the PV of tile j - 2 is done; O is complete before it is rescaled
-      if (j >= 2) w_ok &= __all_sync(0xffffffffu, mbar_wait(&pv_done[pb], (uint32_t)(((j - 2) >> 1) & 1), a.timeout_ns));
-      if (any && j >= 1) {
-        w_ok &= __all_sync(0xffffffffu, mbar_wait(&pv_done[(j - 1) & 1], (uint32_t)(((j - 1) >> 1) & 1), a.timeout_ns));
-        tc_fence_after();
-#pragma unroll
-        for (int h = 0; h < C::HALVES; ++h) {
-          const uint32_t orow = tbase + ((uint32_t)(q * 32) << 16) + O_COL + h * N;
-          float o[16];
-          tmem_ld16(orow, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] *= fac[i];
-          tmem_st16(orow, o);
-        }
-        tmem_st_wait();
-      }
-      uint8_t* prow = smem + C::OFF_P + pb * 2 * C::PLANE_P;
-      float ps[NC];
+      uint8_t* prow = smem + C::OFF_P + pb * C::P_BYTES;
 #pragma unroll
       for (int c = 0; c < NC; c += 2) {
+        float p[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) ps[c + i] = sv[c + i] == -INFINITY ? 0.f : exp2f(sv[c + i] - mref[c + i] + P_SHIFT);
+        for (int i = 0; i < 2; ++i) {
+          p[i] = sv[c + i] == -INFINITY ? 0.f : ex2(sv[c + i] - mref[c + i] + P_SHIFT);
+          lsum[c + i] += p[i];  // of this thread's keys; they are added up at the end
+        }
         uint32_t hi, lo;
-        split2(ps[c], ps[c + 1], hi, lo);
+        split2p(p[0], p[1], hi, lo);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint8_t* dst = prow + (c + i) * 128 + ((((r >> 4) ^ ((c + i) & 7)) << 4) | (r & 15));
           dst[0] = (uint8_t)(hi >> (8 * i));
-          dst[C::PLANE_P] = (uint8_t)(lo >> (8 * i));
+          dst[NC * 128] = (uint8_t)(lo >> (8 * i));
         }
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) ps[c] += __shfl_xor_sync(0xffffffffu, ps[c], o);
-      if (lane == 0) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) rsum[q * N + c] = ps[c];
-      }
-      if (!w_ok && lane == 0) atomicOr(&s_fail, 1);
       fence_proxy_async();
       tc_fence_before();
       mbar_arrive(&p_full[pb]);
-      wd_bar();
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        lsum[c] = lsum[c] * fac[c] + ((rsum[c] + rsum[N + c]) + (rsum[2 * N + c] + rsum[3 * N + c]));
-      if (s_fail) {
-        ok = false;
-        break;
-      }
     }
     if (ok && n > 0) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[(n - 1) & 1], (uint32_t)(((n - 1) >> 1) & 1), a.timeout_ns));
+      // the products of the last two tiles: their barriers are separate
+      ok = warp_wait(&pv_done[(n - 1) & 1], (uint32_t)(((n - 1) >> 1) & 1), a.timeout_ns);
       tc_fence_after();
     }
     if (!ok) report_error(a.status, kErrMbarTimeout, 313, r);
+    wd_bar();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) lsum[c] += __shfl_xor_sync(0xffffffffu, lsum[c], o);
+      if (lane == 0) red[c * 4 + q] = lsum[c];
+    }
     // this CTA's partial results [row][dim], over the ring (all its tiles have been used)
     if (n > 0 && ok) {
       float* part = reinterpret_cast<float*>(smem + C::OFF_RING);
 #pragma unroll
       for (int h = 0; h < C::HALVES; ++h) {
-        float o[16];
-        tmem_ld16(tbase + ((uint32_t)(q * 32) << 16) + O_COL + h * N, o);
+        float o[N];
+#pragma unroll
+        for (int c0 = 0; c0 < N; c0 += 16) tmem_ld16(tbase + ((uint32_t)(q * 32) << 16) + O_COL + h * N + c0, o + c0);
         tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < NC; ++c) part[c * D + h * 128 + r] = o[c];
+        for (int c = 0; c < NC; ++c) part[c * D + h * 128 + r] = o[c] + o[NC + c];
       }
     }
+    wd_bar();
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       if (tr == c) {
+        const float4 l4 = *reinterpret_cast<const float4*>(red + c * 4);
         col_m[c] = n > 0 && ok ? mref[c] : -INFINITY;
-        col_l[c] = n > 0 && ok ? lsum[c] : 0.f;
+        col_l[c] = n > 0 && ok ? (l4.x + l4.y) + (l4.z + l4.w) : 0.f;
+        if (c < NQ && poison[c / a.G]) col_l[c] = __int_as_float(0x7fffffff);
       }
-    wd_bar();
-    if (tr < NQ && poison[tr / a.G]) col_l[tr] = __int_as_float(0x7fffffff);
   }
+  __syncwarp();  // the cluster's barrier wants whole warps
   tc_fence_before();
   if (nsplit > 1) cluster_sync();
   else __syncthreads();
 
-  // each CTA of the cluster joins a share of the dims of every row
+  // each CTA of the cluster joins a share of the dims of every row: the partial results' weights first
   {
-    const int dn = D / nsplit;
     const uint32_t part = smem_u32(smem + C::OFF_RING), ml = smem_u32(col_m);
+    if (threadIdx.x < NQ) {
+      const int row = threadIdx.x;
+      float m[8], l[8], M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < nsplit) {
+          const uint32_t b = mapa_shared(ml, (uint32_t)s);
+          m[s] = ld_dsmem(b + row * 4);
+          l[s] = ld_dsmem(b + (ROWS + row) * 4);
+          if (l[s] != 0.f) M = fmaxf(M, m[s]);
+        }
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < nsplit) {
+          m[s] = l[s] == 0.f ? 0.f : m[s] == -INFINITY ? 1.f : ex2(m[s] - M);
+          if (l[s] != 0.f) L += m[s] * l[s];
+        }
+      const float inv = L != 0.f ? a.v_scale / L : 0.f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s < nsplit) weight[row * 8 + s] = m[s] * inv;
+    }
+    __syncthreads();
+    const int dn = D / 4 / nsplit;  // four dims an item
     for (int i = threadIdx.x; i < NQ * dn; i += THREADS) {
-      const int row = i / dn, d = split * dn + i % dn;
-      float M = -INFINITY, L = 0.f, acc = 0.f;
-      for (int s = 0; s < nsplit; ++s) {
-        const uint32_t b = nsplit > 1 ? mapa_shared(ml, (uint32_t)s) : ml;
-        const float l = ld_dsmem(b + (N + row) * 4);
-        if (l != 0.f) M = fmaxf(M, ld_dsmem(b + row * 4));
-      }
-      for (int s = 0; s < nsplit; ++s) {
-        const uint32_t b = nsplit > 1 ? mapa_shared(ml, (uint32_t)s) : ml;
-        const uint32_t p = nsplit > 1 ? mapa_shared(part, (uint32_t)s) : part;
-        const float l = ld_dsmem(b + (N + row) * 4);
-        if (l == 0.f) continue;
-        const float m = ld_dsmem(b + row * 4);
-        const float w = m == -INFINITY ? 1.f : exp2f(m - M);
-        L += w * l;
-        acc += w * ld_dsmem(p + (row * D + d) * 4);
-      }
-      float o = L != 0.f ? acc / L * a.v_scale : 0.f;
+      const int row = i / dn, d = 4 * (split * dn + i % dn);
       const int tok = tok0 + row / a.G, col = (kvh * a.G + row % a.G) * D + d;
-      if (a.gate != nullptr) o *= sigmoid_f(__bfloat162float(a.gate[(int64_t)tok * a.ld_gate + col]));
-      a.out[(int64_t)tok * a.ld_out + col] = __float2bfloat16(o);
+      uint2 g = make_uint2(0, 0);
+      if (a.gate != nullptr) g = *reinterpret_cast<const uint2*>(a.gate + (int64_t)tok * a.ld_gate + col);
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < nsplit; ++s) {
+        const float w = weight[row * 8 + s];
+        if (w == 0.f) continue;  // nothing was seen there: nothing was written either
+        const float4 v = ld_dsmem_f4(mapa_shared(part, (uint32_t)s) + (row * D + d) * 4);
+        o[0] += w * v.x;
+        o[1] += w * v.y;
+        o[2] += w * v.z;
+        o[3] += w * v.w;
+      }
+      const __nv_bfloat16* ge = reinterpret_cast<const __nv_bfloat16*>(&g);
+      uint2 w2;
+      __nv_bfloat16* we = reinterpret_cast<__nv_bfloat16*>(&w2);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (a.gate != nullptr) o[c] *= sigmoid_f(__bfloat162float(ge[c]));
+        we[c] = __float2bfloat16(o[c]);
+      }
+      *reinterpret_cast<uint2*>(a.out + (int64_t)tok * a.ld_out + col) = w2;
     }
   }
   if (nsplit > 1) cluster_sync();  // peers read this CTA's shared memory until here
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tbase, TMEM_COLS);
+    tmem_dealloc(tbase, C::TMEM_COLS);
   }
 }
 
@@ -721,11 +782,12 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
   const int per = ROWS / a.G;  // tokens of a tile
 
   // the sequence and the tokens of this tile: tiles are numbered through the sequences
-  int seq = -1, tok0 = 0, ntok = 0;
+  int seq = -1, tok0 = 0, ntok = 0, len_seq = 0, start = 0;
   {
     int before = 0;
     for (int s0 = 0; s0 < a.S && seq < 0; s0 += 32) {
       const int len = s0 + lane < a.S ? max(a.seq_len[s0 + lane], 0) : 0;
+      const int st = s0 + lane < a.S ? a.seq_start[s0 + lane] : 0;
       const int tiles = len > a.max_new ? 0 : (len + per - 1) / per;
       int inc = tiles;
 #pragma unroll
@@ -741,7 +803,9 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
         const int first = (int)blockIdx.x - before - (__shfl_sync(0xffffffffu, inc - tiles, src));
         seq = s0 + src;
         tok0 = first * per;
-        ntok = min(per, __shfl_sync(0xffffffffu, len, src) - tok0);
+        len_seq = __shfl_sync(0xffffffffu, len, src);
+        start = __shfl_sync(0xffffffffu, st, src);
+        ntok = min(per, len_seq - tok0);
       }
       before += __shfl_sync(0xffffffffu, inc, 31);
     }
@@ -751,20 +815,34 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
     if (threadIdx.x == 0) report_error(a.status, kErrConfig, 325, (int)smem_u32(smem));
     return;
   }
-  {
-    const int start = a.seq_start[seq], len = a.seq_len[seq];
-    if (start < 0 || start > a.T - len) {
-      if (threadIdx.x == 0) report_error(a.status, kErrBounds, 321, start);
-      return;
-    }
-    tok0 += start;
+  if (start < 0 || start > a.T - len_seq) {
+    if (threadIdx.x == 0) report_error(a.status, kErrBounds, 321, start);
+    return;
   }
+  tok0 += start;
+  const int nrows = ntok * a.G;
+  // softmax warps: this thread's half of its query row, on its way while the CTA is set up
+  constexpr int QC = D / 32;  // 16-element pieces of half a row
+  const int r = (warp & 3) * 32 + lane, half = warp >= 2 ? (warp - 2) >> 2 : 0;
+  const bool valid = warp >= 2 && r < nrows;
+  const int rt = valid ? r / a.G : 0, rg = r % a.G;
+  const int tok = tok0 + rt, head = kvh * a.G + rg;
+  uint4 qraw[QC][2];
+#pragma unroll
+  for (int c = 0; c < QC; ++c) {
+    qraw[c][0] = qraw[c][1] = make_uint4(0, 0, 0, 0);
+    if (valid) {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + head * D) + 2 * (half * QC + c);
+      qraw[c][0] = src[0];
+      qraw[c][1] = src[1];
+    }
+  }
+  const int ctx = valid ? context(a, tok) : 0;
   int ctx_min, ctx_max;
   context_range(a, tok0, ntok, ctx_min, ctx_max);
   const Span sp = make_span(a, ctx_min, ctx_max);
   const int share = (sp.n + nsplit - 1) / nsplit;
   const int j0 = min(sp.n, split * share), n = min(sp.n, j0 + share) - j0;
-  const int nrows = ntok * a.G;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, SOFT);
@@ -793,18 +871,18 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
   auto unit_v = [&](int j) { return SBUF == 1 ? 2 * j + 1 : j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
 
   if (warp == 0) {
-    if (lane == 0) {
-      for (int u = 0; u < 2 * n; ++u) {
+    const bool go = elect_one();
+    Pages pages;
+    for (int u = 0; u < 2 * n; ++u) {
         const bool is_k = SBUF == 1 ? !(u & 1) : u == 0 || ((u & 1) && u < 2 * n - 1);
         const int j = SBUF == 1 ? u / 2 : is_k ? (u + 1) / 2 : u == 2 * n - 1 ? n - 1 : u / 2 - 1;
         const int s = u % C::SLOTS;
-        if (!mbar_wait(&empty[s], (uint32_t)(((u / C::SLOTS) & 1) ^ 1), a.timeout_ns)) {
-          report_error(a.status, kErrMbarTimeout, 322, u);
+        if (!warp_wait(&empty[s], (uint32_t)(((u / C::SLOTS) & 1) ^ 1), a.timeout_ns)) {
+          if (go) report_error(a.status, kErrMbarTimeout, 322, u);
           break;
         }
-        load_tile<D>(a, is_k ? &tmK : &tmV, smem + C::OFF_RING + s * C::UNIT, &full[s], sp, j0 + j, seq, kvh);
+        load_tile<D>(a, is_k ? &tmK : &tmV, smem + C::OFF_RING + s * C::UNIT, &full[s], sp, pages, j0 + j, j0, seq, kvh, go);
       }
-    }
     __syncwarp();
   } else if (warp == 1) {
     if (n > 0) {
@@ -856,35 +934,27 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
     }
     __syncwarp();
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const int r = q * 32 + lane;  // TMEM lane == tile row
-    const bool valid = r < nrows;
-    const int rt = valid ? r / a.G : 0, rg = r % a.G;
-    const int tok = tok0 + rt, head = kvh * a.G + rg;
-    const int ctx = valid ? context(a, tok) : 0;
+    const int q = warp & 3;  // r is the TMEM lane and the tile's row
     const int seen = a.window > 0 ? ctx - a.window : 0;  // keys from here on are in the window
     auto pair_bar = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory"); };  // the two warps of these rows
     float sl2;
     {
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)tok * a.ld_q + head * D);
       float amax = 0.f;
-      if (valid)
-#pragma unroll 4
-        for (int c = 0; c < D / 16; ++c) {
-          const uint4 raw[2] = {src[2 * c], src[2 * c + 1]};
-          amax = fmaxf(amax, amax16(raw));
-        }
+#pragma unroll
+      for (int c = 0; c < QC; ++c) amax = fmaxf(amax, amax16(qraw[c]));
+      red[half * ROWS + r] = amax;
+      pair_bar();
+      amax = fmaxf(amax, red[(half ^ 1) * ROWS + r]);
+      pair_bar();  // red is used again
       const int e = amax > 0.f ? mx_exponent(amax, 448.f) : 0;
       sl2 = fmaxf(fabsf(a.scale_log2) * exp2i(max(e, -126)), 1.17549435e-38f);
       const float inv = copysignf(exp2i(-e), a.scale_log2);  // scores come out with the scale's sign
-#pragma unroll 4
-      for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (valid) {
-          const uint4 raw[2] = {src[2 * c], src[2 * c + 1]};
-          split16(raw, inv, hi, lo);
-        }
-        uint8_t* dst = smem + C::OFF_Q + (c / 8) * (ROWS * 128) + r * 128 + (((c % 8) ^ (r & 7)) << 4);
+#pragma unroll
+      for (int c = 0; c < QC; ++c) {
+        const int pc = half * QC + c;  // 16-byte piece of the row
+        uint4 hi, lo;
+        split16(qraw[c], inv, hi, lo);
+        uint8_t* dst = smem + C::OFF_Q + (pc / 8) * (ROWS * 128) + r * 128 + (((pc % 8) ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(dst) = hi;
         *reinterpret_cast<uint4*>(dst + C::PLANE_Q) = lo;
       }
@@ -904,18 +974,20 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
       // One CTA an SM keeps its 64 scores in registers; two have registers for 32, and read them twice.
       constexpr int PART = C::CTAS == 1 ? HK : HK / 2;
       const uint32_t scol = trow + S_COL + s * KT + half * HK;
-      const int key0 = sp.key0(j0 + j), end = sp.end(j0 + j);
-      const bool whole = key0 + KT <= min(ctx_min, end) && (a.window == 0 || key0 >= ctx_max - a.window);
+      const int key0 = sp.key(2 * (j0 + j) + half);  // of this thread's page
+      const bool whole = whole_page(a, key0, ctx_min, ctx_max);
+      // columns that this row sees: [first, first + count), and those before sink
+      const int first = max(seen - key0, 0), sink = min(a.sinks, ctx) - key0;
+      const uint32_t count = (uint32_t)max(min(ctx - key0, HK) - first, 0);
       float sv[PART];
       auto load = [&](int part) {
 #pragma unroll
         for (int c = 0; c < PART; c += 16) tmem_ld16(scol + part * PART + c, sv + c);
         tmem_ld_wait();
         if (!whole) {
-          const int top = min(ctx, end), first = key0 + half * HK + part * PART;
 #pragma unroll
           for (int c = 0; c < PART; ++c)
-            if (first + c >= top || (first + c < seen && first + c >= a.sinks)) sv[c] = -INFINITY;
+            if ((uint32_t)(part * PART + c - first) >= count && part * PART + c >= sink) sv[c] = -INFINITY;
         }
       };
       float tmax = -INFINITY;
@@ -927,12 +999,15 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
         for (int c = 0; c < PART; ++c) m4[c & 3] = fmaxf(m4[c & 3], sv[c]);
         tmax = fmaxf(tmax, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
       }
-      if (!whole && half < C::HALVES) {
+      // value rows of pages that some row does not see whole: a thread a row and column half
+      const int vkey = sp.key(2 * (j0 + j) + (q >> 1));
+      if (half < C::HALVES && !whole_page(a, vkey, ctx_min, ctx_max)) {
         const int u = unit_v(j);
         ok &= warp_wait(&full[u % C::SLOTS], (uint32_t)((u / C::SLOTS) & 1), a.timeout_ns);
         uint8_t* tile = smem + C::OFF_RING + (u % C::SLOTS) * C::UNIT;
-        if (half == 0) clean_value_row<0, 1>(a, tile, r, key0 + r, end, tok0, ntok, poison);
-        else clean_value_row<C::HALVES - 1, C::HALVES>(a, tile, r, key0 + r, end, tok0, ntok, poison);
+        const int key = vkey + (r & (PAGE - 1));
+        if (half == 0) clean_value_row<0, 1>(a, tile, r, key, tok0, ntok, poison);
+        else clean_value_row<C::HALVES - 1, C::HALVES>(a, tile, r, key, tok0, ntok, poison);
         fence_proxy_async();  // the product reads the cleared rows
       }
       red[((j & 1) * 2 + half) * ROWS + r] = ok ? tmax : __int_as_float(0x7fffffff);
@@ -990,12 +1065,21 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
         }
       }
       tmem_st_wait();
+      // A parity tells neighbouring phases apart only. The wait after the loop is for the last product, so the
+      // one before it is waited for here, where the last cannot have run yet.
+      if (SBUF == 2 && j == n - 1 && j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
       tc_fence_before();
       mbar_arrive(p_full);
     }
-    // S(n - 1) came after PV(n - 1 - SBUF), so up to two products are still to come: one phase at a time, since
-    // a parity does not tell the last from the one before the last but one
-    if (SBUF == 2 && n > 1 && ok) ok = warp_wait(pv_done, (uint32_t)((n - 2) & 1), a.timeout_ns);
+    uint4 graw[QC][2] = {};  // the gate of this thread's half of the output, on its way during the last product
+    if (nsplit == 1 && valid && a.gate != nullptr) {
+      const uint4* g = reinterpret_cast<const uint4*>(a.gate + (int64_t)tok * a.ld_gate + head * D + half * (D / 2));
+#pragma unroll
+      for (int c = 0; c < QC; ++c) {
+        graw[c][0] = g[2 * c];
+        graw[c][1] = g[2 * c + 1];
+      }
+    }
     if (n > 0 && ok) ok = warp_wait(pv_done, (uint32_t)((n - 1) & 1), a.timeout_ns);
     tc_fence_after();
     if (!ok) report_error(a.status, kErrMbarTimeout, 324, r);
@@ -1009,32 +1093,28 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
       pair_bar();
       l += row_l[(half ^ 1) * ROWS + r];
       const float inv = have && l != 0.f ? a.v_scale / l : 0.f;
-#pragma unroll 1
-      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 16) {
+#pragma unroll
+      for (int c = 0; c < QC; ++c) {
+        const int col = half * (D / 2) + 16 * c;
         float o[16];
         if (have) {
-          tmem_ld16(trow + O_COL + c, o);
+          tmem_ld16(trow + O_COL + col, o);
           tmem_ld_wait();
         }
-        if (!valid) continue;
+        const __nv_bfloat16* ge = reinterpret_cast<const __nv_bfloat16*>(graw[c]);
         uint4 w[2];
         __nv_bfloat16* we = reinterpret_cast<__nv_bfloat16*>(w);
-        uint4 gr[2] = {};
-        if (a.gate != nullptr) {
-          const uint4* g = reinterpret_cast<const uint4*>(a.gate + (int64_t)tok * a.ld_gate + head * D + c);
-          gr[0] = g[0];
-          gr[1] = g[1];
-        }
-        const __nv_bfloat16* ge = reinterpret_cast<const __nv_bfloat16*>(gr);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float v = inv != 0.f ? o[i] * inv : 0.f;  // O of a row without weights was never written
           if (a.gate != nullptr) v *= sigmoid_f(__bfloat162float(ge[i]));
           we[i] = __float2bfloat16(v);
         }
-        uint4* dst = reinterpret_cast<uint4*>(a.out + (int64_t)tok * a.ld_out + head * D + c);
-        dst[0] = w[0];
-        dst[1] = w[1];
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(a.out + (int64_t)tok * a.ld_out + head * D + col);
+          dst[0] = w[0];
+          dst[1] = w[1];
+        }
       }
     } else {
       // partial results over the ring: row r's 16-byte pieces at c ^ (r & 31), so that a warp's
@@ -1051,6 +1131,7 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
       }
     }
   }
+  __syncwarp();  // the cluster's barrier wants whole warps
   tc_fence_before();
   if (nsplit > 1) {
     cluster_sync();
@@ -1160,7 +1241,7 @@ void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
   TORCH_CHECK(max_new >= 1 && max_ctx >= 1, "window_attention: max_new and max_ctx are >= 1");
   TORCH_CHECK(status.device() == q.device() && status.dtype() == torch::kInt32 && status.numel() >= 4, "window_attention: status");
   TORCH_CHECK(T * Hq * D <= ((int64_t)1 << 40) && T <= INT_MAX && S <= 65535 && max_new <= INT_MAX && Hq <= 65535 &&
-                  block_table.size(1) <= (1 << 24) && k_cache.size(0) * Hkv * wa::PAGE <= INT_MAX,
+                  block_table.size(1) <= (1 << 23) && k_cache.size(0) * Hkv * wa::PAGE <= INT_MAX,
               "window_attention: sizes out of range");
   if (T == 0 || S == 0) return;
   const at::cuda::CUDAGuard guard(q.device());
@@ -1196,11 +1277,11 @@ void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
   const CUtensorMap tk = tmap_u8_kmajor(k_cache.data_ptr(), k_cache.size(0) * Hkv * wa::PAGE, D, wa::PAGE);
   const CUtensorMap tv = tmap_u8_kmajor(v_cache.data_ptr(), v_cache.size(0) * Hkv * wa::PAGE, D, wa::PAGE);
   // tiles of keys that one group of rows can see at most
-  const int64_t span = window > 0 ? std::min(max_ctx, window + sinks + a.max_new + 2 * wa::KT) : max_ctx;
+  const int64_t span = window > 0 ? std::min(max_ctx, window + sinks + a.max_new + 2 * wa::PAGE) : max_ctx;
   const int64_t tiles = (span + wa::KT - 1) / wa::KT;
   const int64_t sms = device_sm_count();
   const int64_t nq = (int64_t)a.max_new * a.G;  // rows of the longest sequence and one kv head
-  const bool dec = nq <= wd::N;
+  const bool dec = nq <= wd::ROWS;
   const int64_t per = wc::ROWS / a.G;
   const int64_t groups = dec ? S : std::min(T / per + S, S * ((a.max_new + per - 1) / per));
   // CTAs of a cluster share a group's keys while that fills the GPU and leaves each of them a tile
@@ -1210,11 +1291,11 @@ void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
   TORCH_CHECK(groups <= INT_MAX, "window_attention: too many rows");
   if (dec) {
     if (D == 128) {
-      if (nq <= 8) launch_cluster(window_attn_dec_kernel<128, 8>, wd::Cfg<128>::SMEM, grid, wd::THREADS, tk, tv, a);
-      else launch_cluster(window_attn_dec_kernel<128, 16>, wd::Cfg<128>::SMEM, grid, wd::THREADS, tk, tv, a);
+      if (nq <= 8) launch_cluster(window_attn_dec_kernel<128, 8>, wd::Cfg<128, 8>::SMEM, grid, wd::THREADS, tk, tv, a);
+      else launch_cluster(window_attn_dec_kernel<128, 16>, wd::Cfg<128, 16>::SMEM, grid, wd::THREADS, tk, tv, a);
     } else {
-      if (nq <= 8) launch_cluster(window_attn_dec_kernel<256, 8>, wd::Cfg<256>::SMEM, grid, wd::THREADS, tk, tv, a);
-      else launch_cluster(window_attn_dec_kernel<256, 16>, wd::Cfg<256>::SMEM, grid, wd::THREADS, tk, tv, a);
+      if (nq <= 8) launch_cluster(window_attn_dec_kernel<256, 8>, wd::Cfg<256, 8>::SMEM, grid, wd::THREADS, tk, tv, a);
+      else launch_cluster(window_attn_dec_kernel<256, 16>, wd::Cfg<256, 16>::SMEM, grid, wd::THREADS, tk, tv, a);
     }
   } else if (D == 128) {
     launch_cluster(window_attn_chunk_kernel<128>, wc::Cfg<128>::SMEM, grid, wc::THREADS, tk, tv, a);

@@ -91,6 +91,13 @@ def test_chunks(hq, hkv, d, window, sinks):
     _check(_case([0, 200, 129, 400], [190, 67, 1, 43], hq, hkv, d, seed=2), window, sinks)
 
 
+@pytest.mark.parametrize("gate", [False, True])
+def test_wide_chunk_over_a_long_window(gate):
+    """Enough tiles that nothing is split, many key tiles each."""
+    _check(_case([3001, 1777], [260, 233], 24, 4, 256, seed=12, gate=gate), 2048, 4, max_new=260)
+    _check(_case([1500, 777], [300, 333], 32, 8, 128, seed=13, gate=gate), 1024, 130)
+
+
 def test_long_context_split():
     """A few rows against a long cache (the work is split over the keys and joined)."""
     for window, sinks, new in [(0, 0, 1), (3000, 5, 1), (2500, 700, 9), (0, 0, 30)]:
@@ -163,6 +170,17 @@ def test_nan_in_a_visible_key_stays_with_the_rows_that_see_it(new):
     out = _run(c, 0, 0)
     assert bool(out[new // 2: new].isnan().all())
     assert torch.equal(out[: new // 2], want[: new // 2]) and torch.equal(out[new:], want[new:])
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_nan_in_a_query_stays_in_its_row(new):
+    c = _case([200, 200], [new, new], 6, 1, 128, seed=8, gate=False)
+    want = _run(c, 0, 0)
+    c["q"][new, 2, 5] = float("nan")
+    out = _run(c, 0, 0).view(-1, 6, 128)
+    assert bool(out[new, 2].isnan().all())
+    out[new, 2] = want.view(-1, 6, 128)[new, 2]
+    assert torch.equal(out.view_as(want), want)
 
 
 def test_other_stream_and_graph():
