@@ -234,6 +234,17 @@ R9K_DEVINL float as_logit(__nv_bfloat16 v) { return as_logit(__bfloat162float(v)
 template <typename T>
 R9K_DEVINL int lead(const T* src) { return (int)(((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / sizeof(T)); }
 
+// The part of a slice's 16-byte loads that a warp takes: neighbouring ones, so that the warps' sums are in
+// index order (the entries before the first boundary go to the first warp, those after the last to the last).
+struct Share {
+  int lo, hi;
+  R9K_DEVINL Share(int vecs, int warp) {
+    const int per = (vecs + WARPS - 1) / WARPS;
+    lo = min(vecs, warp * per);
+    hi = min(vecs, lo + per);
+  }
+};
+
 // Every logit i < n of a slice in global or shared memory, a thread each: four(x, i) for four at a time
 // from the first 16-byte boundary on (four loads in flight), one(x, i) for those around them.
 template <typename T, typename F1, typename F4>
@@ -250,19 +261,19 @@ R9K_DEVINL void scan(const T* src, int n, F1 one, F4 four) {
       four(x, head + v * VEC + i);
     }
   };
-  int v = threadIdx.x;
-  for (; v + 3 * THREADS < vecs; v += 4 * THREADS) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Share mine(vecs, warp);
+  int v = mine.lo + lane;
+  for (; v + 96 < mine.hi; v += 128) {
     uint4 raw[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) raw[j] = body[v + j * THREADS];
+    for (int j = 0; j < 4; ++j) raw[j] = body[v + 32 * j];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) each(raw[j], v + j * THREADS);
+    for (int j = 0; j < 4; ++j) each(raw[j], v + 32 * j);
   }
-  for (; v < vecs; v += THREADS) each(body[v], v);
-  for (int i = threadIdx.x; i < head + n - rest; i += THREADS) {
-    const int at = i < head ? i : rest + i - head;
-    one(as_logit(src[at]), at);
-  }
+  for (; v < mine.hi; v += 32) each(body[v], v);
+  if (warp == 0 && lane < head) one(as_logit(src[lane]), lane);
+  if (warp == WARPS - 1 && lane < n - rest) one(as_logit(src[rest + lane]), rest + lane);
 }
 template <typename T, typename F>
 R9K_DEVINL void scan(const T* src, int n, F f) {
@@ -632,8 +643,7 @@ __global__ void __launch_bounds__(sm::THREADS, HELD ? 2 : 3) sample_kernel(const
         if (me != 0) return;
         const int m = min((int)sh.listed, CAP);
         const u64 all = cut == 1 ? sh.last : 0ull;
-        if (m > 256) finish_list(a, r, row, m, all, list, &sh);
-        else if (tid < 32 && m > 128) finish_short<8>(a, r, row, m, all, list);
+        if (m > 128) finish_list(a, r, row, m, all, list, &sh);
         else if (tid < 32 && m > 64) finish_short<4>(a, r, row, m, all, list);
         else if (tid < 32) finish_short<2>(a, r, row, m, all, list);
         return;
@@ -662,21 +672,32 @@ __global__ void __launch_bounds__(sm::THREADS, HELD ? 2 : 3) sample_kernel(const
     }
   }
 
-  // weights of the kept tokens, a slice a CTA; the draw in index order
+  // weights of the kept tokens, a slice a CTA and a part of it a warp; the draw in index order
   u64 sum = 0;
   scan(xs, n, [&](float x, int i) {
     if (full_key(x, i0 + i) <= last && r.e(x) >= r.min_p) sum += r.w(x);
   });
+  u64 part = sum;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+  if ((tid & 31) == 0) sh.warp2[tid >> 5] = part;
   u64 base;
   const u64 total = cluster_join(sum, SUM, &sh, round, &base);
   const double at = floor((double)a.u[row] * (double)total);
   u64 target = at > 0. ? (u64)at : 0ull;  // a NaN draws the first
   if (target > total - 1) target = total - 1;
   if (target < base) return;
-  for (int c = 0; c < n && base <= target; c += THREADS) {  // running sums of 512 indexes at a time
+  int w0 = 0;
+  while (w0 < WARPS && base + sh.warp2[w0] <= target) base += sh.warp2[w0++];
+  if (w0 == WARPS) return;  // a later CTA's
+  constexpr int VEC = 16 / sizeof(U);
+  const int head = min(n, lead(xs)), vecs = (n - head) / VEC;
+  const Share share(vecs, w0);
+  const int end = w0 == WARPS - 1 ? n : head + share.hi * VEC;
+  for (int c = w0 == 0 ? 0 : head + share.lo * VEC; c < end && base <= target; c += THREADS) {  // 512 indexes at a time
     const int i = c + tid;
     u64 w = 0;
-    if (i < n) {
+    if (i < end) {
       const float x = as_logit(xs[i]);
       if (full_key(x, i0 + i) <= last && r.e(x) >= r.min_p) w = r.w(x);
     }
@@ -708,23 +729,24 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   if (min_p.has_value()) chk(*min_p, torch::kFloat32, "min_p");
   chk(tokens, torch::kInt64, "tokens");
   chk(logprobs, torch::kFloat32, "logprobs");
+  constexpr int HELD_SLICE = 25600;  // two CTAs an SM
   constexpr int MAX_SLICE = 65532;  // a histogram's halves of weights sum to 32 bits
   TORCH_CHECK(V <= (int64_t)sm::MAX_CLUSTER * MAX_SLICE, "sample_logits: vocabulary too large");
   if (R == 0) return;
   const at::cuda::CUDAGuard guard(logits.device());
-  // The most CTAs a row that still let all rows run in one wave (three CTAs an SM, of which clusters of 16
-  // leave a quarter unused), a slice of at least 4096; where no count does, the fewest. Measured, CTAs a row
-  // x 16 / 8 / 4: 256 rows x 248320 fp32, top-k, 250 / 158 / 141 us; 64 rows 84 / 61 / -; 64 rows x 100003,
-  // top-p, - / 66 / 47 us.
+  // The most CTAs a row that still let all rows run in one wave, a slice of at least 4096; where no count does,
+  // the fewest. A wave is three CTAs an SM for slices read twice, two for held ones (below), and clusters leave
+  // some of it unused. Measured, CTAs a row x 16 / 8 / 4: 256 rows x 248320 fp32, top-k, 250 / 158 / 124 us; 64
+  // rows 84 / 61 / -; 16 rows 35 / 30 / -; 64 rows x 100003 bf16, top-p, 86 / 59 / 54 us.
   const int64_t sms = device_sm_count();
   auto slice_of = [&](int c) { return ((V + c - 1) / c + 3) / 4 * 4; };
   int least = 1;
   while (slice_of(least) > 65532) least *= 2;
   int C = sm::MAX_CLUSTER;
-  while (C > least && (slice_of(C) < 4096 || R * C > (C == 16 ? sms * 9 / 4 : sms * 5 / 2))) C /= 2;
+  while (C > least && (slice_of(C) < 4096 || R * C > (C == 16 ? sms * 3 / 2 : sms * 5 / 2))) C /= 2;
   // Slices held in shared memory are read once, but leave room for two CTAs an SM: while that wave takes
-  // all rows too (64 x 100003, 4 CTAs a row: 45 us held, 47 not; 16 x 248320, 16 CTAs: 37 us held, 28 not).
-  const bool held = slice_of(C) <= 25000 && R * C <= (C == 16 ? sms * 3 / 2 : sms * 7 / 4);
+  // all rows too (64 x 100003 bf16, 4 CTAs a row: 54 us held, 68 not; one row, 16 CTAs: 13.7 held, 15.4 not).
+  const bool held = slice_of(C) <= HELD_SLICE && R * C <= (C == 16 ? sms * 3 / 2 : sms * 7 / 4);
   TORCH_CHECK(R * C <= INT_MAX, "sample_logits: too many rows");
   sm::Args a{logits.data_ptr(), logits.stride(0), (int)V, (int)slice_of(C), u.data_ptr<float>(),
              temperature.data_ptr<float>(), top_k.has_value() ? top_k->data_ptr<int32_t>() : nullptr,
@@ -734,7 +756,7 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   const bool f32 = logits.dtype() == torch::kFloat32;
   auto kern = held ? (f32 ? sample_kernel<float, true> : sample_kernel<__nv_bfloat16, true>)
                    : (f32 ? sample_kernel<float, false> : sample_kernel<__nv_bfloat16, false>);
-  TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + (held ? 25000 * 4 + 16 : 0)) == cudaSuccess &&
+  TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + (held ? HELD_SLICE * 4 + 16 : 0)) == cudaSuccess &&
                   cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess,
               "sample_logits: kernel attributes");
   cudaLaunchConfig_t cfg = {};
