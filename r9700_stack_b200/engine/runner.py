@@ -299,10 +299,11 @@ class ModelRunner:
         return res
 
     def _resample(self, hot, res) -> None:
-        from .sampler import sample_rows
+        from .sampler import sample_rows, sample_rows_device
 
         rows = torch.tensor([r for r, _ in hot], device=self.device)
-        new = sample_rows(self.ws.logits.index_select(0, rows), [s.params for _, s in hot],
+        draw = sample_rows_device if self.cfg.device_sampling else sample_rows
+        new = draw(self.ws.logits.index_select(0, rows), [s.params for _, s in hot],
                           [len(s.output) for _, s in hot])
         for (_, s), t in zip(hot, new):
             res[s.seq_id] = [t]

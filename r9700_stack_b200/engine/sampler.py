@@ -4,6 +4,10 @@ Greedy rows (temperature 0) take the argmax; the runner folds that into the capt
 Sampled rows apply temperature, top-k and top-p (nucleus) filtering and draw from the renormalised
 distribution with a per-request generator (``SamplingParams.seed`` + tokens generated so far), so a
 request's samples do not depend on which other requests share its batch.
+
+``sample_rows_device`` does the same for all rows in one launch (``EngineConfig.device_sampling``): each
+row's uniform number comes from its request's seed and the tokens generated so far, and equal logits
+rank by index. Its draws are other draws of the same distributions.
 """
 from __future__ import annotations
 
@@ -39,7 +43,38 @@ def sample_rows(logits: torch.Tensor, params_list, steps: list[int]) -> list[int
             sx = sx.masked_fill(drop, float("-inf"))
             x = torch.full_like(x, float("-inf")).scatter(0, si, sx)
         prob = torch.softmax(x, -1)
+        if p.min_p > 0:
+            prob = torch.where(prob >= min(p.min_p, 1.0) * prob.max(), prob, 0.0)
         gen = torch.Generator(device=logits.device)
         gen.manual_seed((p.seed * 1000003 + steps[i]) & 0x7FFFFFFFFFFFFFFF)
         out[i] = int(torch.multinomial(prob, 1, generator=gen))
     return out
+
+
+def uniform(seed: int, step: int) -> float:
+    """A number in [0, 1) with 24 random bits, of (seed, step) alone: two rounds of the splitmix64 mix
+    (Steele, Lea and Flood, 2014)."""
+    mask = (1 << 64) - 1
+    z = ((seed & mask) * 0x9E3779B97F4A7C15 + step) & mask
+    for _ in range(2):
+        z = (z + 0x9E3779B97F4A7C15) & mask
+        z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & mask
+        z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & mask
+        z ^= z >> 31
+    return (z >> 40) / float(1 << 24)
+
+
+def device_params(params_list, device):
+    """(temperature, top_k, top_p, min_p) of one request a row, as ``ops.sampling.sample_tokens`` takes them."""
+    f = lambda name: torch.tensor([float(getattr(p, name)) for p in params_list], dtype=torch.float32, device=device)
+    k = torch.tensor([p.top_k for p in params_list], dtype=torch.int32, device=device)
+    return f("temperature"), k, f("top_p"), f("min_p")
+
+
+def sample_rows_device(logits: torch.Tensor, params_list, steps: list[int]) -> list[int]:
+    """As :func:`sample_rows`, in one launch. A row with nothing to draw from (no number above -inf) gives 0."""
+    from ..ops.sampling import sample_tokens
+
+    u = torch.tensor([uniform(p.seed, s) for p, s in zip(params_list, steps)], dtype=torch.float32, device=logits.device)
+    tokens, _ = sample_tokens(logits, u, *device_params(params_list, logits.device))
+    return tokens.clamp_min(0).tolist()

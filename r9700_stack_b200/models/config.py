@@ -52,6 +52,10 @@ class HybridConfig:
     # indexer of qsa_heads x 128 query heads against mean-pooled group keys (0 = dense attention)
     qsa_topk: int = 0
     qsa_heads: int = 4
+    # sliding window of the full-attention layers, in tokens, and the first tokens of a sequence that stay
+    # visible (0 = the whole context)
+    attn_window: int = 0
+    attn_sinks: int = 0
     # hyper-connections: HC residual streams, sigmoid-gated mix into every block (0 = plain residual)
     hc_streams: int = 0
     init_std: float = 0.02
@@ -216,3 +220,4 @@ class EngineConfig:
     spec_tokens: int = 0  # draft tokens verified per step (0: no speculative decoding)
     spec_method: str = "ngram"  # ngram | mtp | block | dspark
     ep_placement: str = ""  # JSON expert placement (parallel.ep_placement) for MoE models; "" = contiguous
+    device_sampling: bool = False  # requests that sample draw on the device (ops.sampling), all rows in one launch

@@ -21,6 +21,7 @@ import torch
 
 from .. import _native, knobs
 from ..ops import linear as L
+from ..ops.window_attention import window_attention
 from .config import HybridConfig, ParallelConfig
 from ..utils import status as _status
 from .weights import TPFactory, WeightFactory, from_float
@@ -151,6 +152,8 @@ class HybridLM:
         self.gdn_dims = dict(hk=hk, hv=hv, conv_ch=2 * hk * d + hv * d, proj_rows=2 * hk * d + 2 * hv * d + 2 * hv)
         self.ffn_local = c.ffn // tp if c.ffn else 0
         assert c.vocab % tp == 0
+        if c.attn_window and (c.qsa_topk or c.head_dim not in (128, 256)):
+            raise ValueError("attn_window: head_dim 128 or 256, and no QSA selection beside it")
         self.vocab_local = c.vocab // tp
         self.sm_scale = 1.0 / math.sqrt(c.head_dim)
         self.k_scale = 1.0
@@ -338,6 +341,15 @@ class HybridLM:
                                   ws.q[:T], kc, vc, self.k_scale, self.v_scale)
         gate = qkv[:, gate_off:gate_off + hq * D] if gate_off >= 0 else None
         if c.qsa_topk and self._qsa(i, lay, meta, ws, T, gate):
+            if self.mx:
+                L.quant_act(ws.attn_bf16[:T], out=ws.attn_act.narrow(T))
+            return ws.attn_act.narrow(T), ws.attn_bf16[:T], lay["w_o"]
+        if c.attn_window:
+            # the captured decode graph has one token a sequence and no host lengths
+            window_attention(ws.q[:T], kc, vc, meta.block_table, meta.seq_start, meta.seq_len, meta.tok_ctx[:T],
+                             self.sm_scale, window=c.attn_window, sinks=c.attn_sinks, k_scale=self.k_scale,
+                             v_scale=self.v_scale, gate=gate, out=ws.attn_bf16[:T], max_ctx=meta.host_max_ctx,
+                             max_new=max(n for _, n in meta.host_seqs) if meta.host_seqs else 1)
             if self.mx:
                 L.quant_act(ws.attn_bf16[:T], out=ws.attn_act.narrow(T))
             return ws.attn_act.narrow(T), ws.attn_bf16[:T], lay["w_o"]

@@ -187,6 +187,8 @@ def _attn(model, i, lay, h, pos, st, mx):
     qpos = pos[:, None]
     kpos = torch.arange(ctx, device=h.device)[None, :]
     allowed = kpos <= qpos
+    if c.attn_window:
+        allowed = allowed & ((kpos > qpos - c.attn_window) | (kpos < c.attn_sinks))
     if c.qsa_topk:
         allowed = allowed & _qsa_mask(model, i, lay, h, pos, st, mx, ctx)
     s = s.masked_fill((~allowed)[:, None, :], float("-inf"))

@@ -30,6 +30,9 @@ def parse(argv=None):
     ap.add_argument("--spec", default="none", choices=["none", "ngram", "mtp", "block", "dspark"])
     ap.add_argument("--ep-placement", default="", help="JSON expert placement (parallel.ep_placement) for MoE models")
     ap.add_argument("--spec-tokens", type=int, default=0)
+    ap.add_argument("--attn-window", type=int, default=0, help="sliding window of the attention layers (0: whole context)")
+    ap.add_argument("--attn-sinks", type=int, default=0, help="first tokens that stay visible beside the window")
+    ap.add_argument("--device-sampling", action="store_true", help="draw sampled tokens on the device, all rows in one launch")
     ap.add_argument("--graph-sizes", default="1,2,4,8,16")
     ap.add_argument("--no-graphs", action="store_true")
     ap.add_argument("--tokenizer", default="", help="local Hugging Face tokenizer directory (default: bytes)")
@@ -39,10 +42,19 @@ def parse(argv=None):
     return ap.parse_args(argv)
 
 
+def windowed(cfg, a):
+    """The model's config with the command line's attention window, which hybrid models have."""
+    if not a.attn_window and not a.attn_sinks:
+        return cfg
+    if not hasattr(cfg, "attn_window") or a.attn_window < 1 or a.attn_sinks < 0:
+        raise SystemExit("--attn-window / --attn-sinks: a hybrid model, a window of at least 1 and sinks >= 0")
+    return cfg.scaled(attn_window=a.attn_window, attn_sinks=a.attn_sinks)
+
+
 def plan(a) -> dict:
     from ..models.config import EngineConfig, model_config
 
-    cfg = model_config(a.model)
+    cfg = windowed(model_config(a.model), a)
     world = int(os.environ.get("WORLD_SIZE", "1"))
     k = a.spec_tokens if a.spec != "none" else 0
     if a.spec != "none" and k == 0:
@@ -50,7 +62,8 @@ def plan(a) -> dict:
     ec = EngineConfig(max_batch=a.max_batch, max_model_len=a.max_model_len, max_prefill_tokens=a.max_prefill_tokens,
                       num_kv_blocks=a.kv_blocks, cuda_graphs=not a.no_graphs,
                       graph_batch_sizes=[int(x) for x in a.graph_sizes.split(",") if x],
-                      spec_tokens=k, spec_method=a.spec if a.spec != "none" else "ngram", ep_placement=a.ep_placement)
+                      spec_tokens=k, spec_method=a.spec if a.spec != "none" else "ngram", ep_placement=a.ep_placement,
+                      device_sampling=a.device_sampling)
     blocks = ec.num_kv_blocks or (ec.max_batch * math.ceil(ec.max_model_len / ec.kv_block) + 1)
     if hasattr(cfg, "attn_layers"):  # hybrid GDN / attention
         hkv = max(1, cfg.n_kv_heads // world)

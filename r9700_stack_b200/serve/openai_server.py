@@ -25,6 +25,7 @@ def _params(body: dict, tok) -> SamplingParams:
     ignore_eos = bool(body.get("ignore_eos", False))
     return SamplingParams(max_tokens=mt, temperature=float(body.get("temperature", 0.0) or 0.0),
                           top_k=int(body.get("top_k", 0) or 0), top_p=float(body.get("top_p", 1.0) or 1.0),
+                          min_p=float(body.get("min_p", 0.0) or 0.0),
                           ignore_eos=ignore_eos, eos_token_id=tok.eos_token_id, seed=int(body.get("seed", 0) or 0))
 
 
