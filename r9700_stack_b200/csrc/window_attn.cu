@@ -7,10 +7,13 @@
 // hold.
 //
 // Precision. The cache stays e4m3 in shared memory, where the MMA reads it; the other operand of each
-// product is the sum of two e4m3 numbers, both multiplied into the same fp32 accumulator: a query q as
-// hi + lo after a power-of-two scaling of its row (exact for |q| >= amax / 1792, else within
-// 2^-19 amax), a probability p as hi + lo (within 2^-8 of itself, or 2^-16 of the row's largest). Two
-// e4m3 products cost what one bf16 product does, and no key or value has to be widened on the way.
+// product is the sum of two 8-bit numbers, both multiplied into fp32 accumulators: a query q as two e4m3
+// numbers after a power-of-two scaling of its row (exact for |q| >= amax / 1792, else within 2^-17 amax),
+// a probability p as an e4m3 number and what that leaves, within 2^-7 of itself (rms 2^-10) or 2^-19 of the
+// row's largest. The rest has a wider range than the first number: e5m2 where both share an accumulator,
+// e4m3 of 16 times itself where each has its own. A first token that takes most of the weight (a sink)
+// leaves the others weights of 2^-14, of which an e4m3 rest would keep two bits. Two 8-bit products cost
+// what one bf16 product does, and no key or value has to be widened on the way.
 //
 // KV cache layout: [pages][kv_heads][64][head_dim] e4m3 for K and V separately.
 #include <torch/extension.h>
@@ -206,13 +209,15 @@ R9K_DEVINL void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   lo = e4m3x2(x - b.x, y - b.y);
 }
 
-// the same for probabilities (0..448): by way of f16, whose conversions are cheaper and whose 2^-12 is far
-// below the lo part's
+// The same for probabilities (0..448): by way of f16, whose conversions are cheaper and whose 2^-12 (2^-25
+// below 2^-14) is far below the rest's. E5M2: the rest as e5m2; else as e4m3 of 16 times itself.
+template <bool E5M2>
 R9K_DEVINL void split2p(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __half2 p = __floats2half2_rn(x, y);
   hi = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(__half2_raw(p), __NV_SATFINITE, __NV_E4M3);
-  const __half2 rest = __hsub2(p, __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)hi, __NV_E4M3)));
-  lo = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(__half2_raw(rest), __NV_SATFINITE, __NV_E4M3);
+  __half2 rest = __hsub2(p, __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)hi, __NV_E4M3)));
+  if (!E5M2) rest = __hmul2(rest, __float2half2_rn(16.f));
+  lo = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(__half2_raw(rest), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
 R9K_DEVINL float ex2(float x) {
   float y;
@@ -243,8 +248,9 @@ R9K_DEVINL float amax16(const uint4 (&r)[2]) {
 }
 
 // Probabilities are exp2(s - m_ref + P_SHIFT): m_ref follows the running maximum once that has grown by
-// P_LAG (O is rescaled then), so the largest lies in [2^6.5, 2^8.75], below e4m3's 448, and the lo
-// part's 2^-10 is 2^-16.5 of it or less.
+// P_LAG (O is rescaled then), so the largest lies in [2^6.5, 2^8.75], below e4m3's 448. Below 2^-6 the
+// first number has steps of 2^-9; the rest, 2^-10 at most, is held to 2^-13 (e5m2) or 2^-14, which is
+// 2^-19 of the largest or less.
 constexpr float P_SHIFT = 6.5f, P_LAG = 2.25f;
 
 // One value row (key r of a tile, column halves [H0, H1)) whose key some of the rows do not see. A NaN code
@@ -597,7 +603,7 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
           lsum[c + i] += p[i];  // of this thread's keys; they are added up at the end
         }
         uint32_t hi, lo;
-        split2p(p[0], p[1], hi, lo);
+        split2p<false>(p[0], p[1], hi, lo);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint8_t* dst = prow + (c + i) * 128 + ((((r >> 4) ^ ((c + i) & 7)) << 4) | (r & 15));
@@ -632,7 +638,7 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
         for (int c0 = 0; c0 < N; c0 += 16) tmem_ld16(tbase + ((uint32_t)(q * 32) << 16) + O_COL + h * N + c0, o + c0);
         tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < NC; ++c) part[c * D + h * 128 + r] = o[c] + o[NC + c];
+        for (int c = 0; c < NC; ++c) part[c * D + h * 128 + r] = o[c] + o[NC + c] * 0.0625f;
       }
     }
     wd_bar();
@@ -887,7 +893,9 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
   } else if (warp == 1) {
     if (n > 0) {
       constexpr uint32_t idesc_s = idesc_dense(kFmtE4M3, kFmtE4M3, ROWS, KT);
-      constexpr uint32_t idesc_o = idesc_dense(kFmtE4M3, kFmtE4M3, ROWS, D) | (1u << 16);  // B (V) MN-major
+      // B (V) MN-major; A is P's e4m3 plane, then its e5m2 plane
+      constexpr uint32_t idesc_o[2] = {idesc_dense(kFmtE4M3, kFmtE4M3, ROWS, D) | (1u << 16),
+                                       idesc_dense(kFmtE5M2, kFmtE4M3, ROWS, D) | (1u << 16)};
       const bool go = elect_one();
       const uint64_t q_desc = sdesc_k_sw128(smem_u32(smem + C::OFF_Q));
       const uint64_t k_desc = sdesc_k_sw128(smem_u32(smem + C::OFF_RING));
@@ -925,7 +933,7 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
         for (int k = 0; k < 4; ++k)
 #pragma unroll
           for (int pl = 0; pl < 2; ++pl)
-            mma_ts(tbase + O_COL, p + pl * 32 + 8 * k, vd + (k * 4096 >> 4), idesc_o, j > 0 || k > 0 || pl > 0, go);
+            mma_ts(tbase + O_COL, p + pl * 32 + 8 * k, vd + (k * 4096 >> 4), pl == 0 ? idesc_o[0] : idesc_o[1], j > 0 || k > 0 || pl > 0, go);
         commit(pv_done, go);
         commit(&empty[u % C::SLOTS], go);
         if (SBUF == 1 && j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
@@ -1024,7 +1032,7 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
       if (need || m_ref == -INFINITY) m_ref = tmax;
       const float off = m_ref == -INFINITY ? 0.f : P_SHIFT - m_ref;  // a row that has seen no key: exp2(-inf) = 0
       float ls[2] = {0.f, 0.f};
-      float ph[HK / 4], pl[HK / 4];  // four e4m3 numbers each
+      float ph[HK / 4], pl[HK / 4];  // four 8-bit numbers each
 #pragma unroll
       for (int part = 0; part < HK / PART; ++part) {
         if (PART < HK) load(part);
@@ -1036,8 +1044,8 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
           ls[0] += p[0] + p[1];
           ls[1] += p[2] + p[3];
           uint32_t h0, l0, h1, l1;
-          split2p(p[0], p[1], h0, l0);
-          split2p(p[2], p[3], h1, l1);
+          split2p<true>(p[0], p[1], h0, l0);
+          split2p<true>(p[2], p[3], h1, l1);
           ph[(part * PART + c) / 4] = __uint_as_float(h0 | (h1 << 16));
           pl[(part * PART + c) / 4] = __uint_as_float(l0 | (l1 << 16));
         }
@@ -1052,7 +1060,7 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
         // S(j) came after PV(j - SBUF): with two S buffers this product may not be done
         if (SBUF == 2 && j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
         tc_fence_after();
-#pragma unroll 1
+#pragma unroll (C::CTAS == 1 ? 2 : 1)
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
           float o[32];
           tmem_ld16(trow + O_COL + c, o);

@@ -51,7 +51,8 @@ def plan_step(new_len, state, block_table, ring, cap: int, *, window: int = 0, s
     if out is None:
         out = torch.empty(plan_numel(cap, seqs), dtype=torch.int32, device=new_len.device)
     _native.ops().plan_step(new_len, state, block_table, ring, cap, window, sinks, out)
-    return StepPlan(*out.split([cap, cap, cap, cap, seqs, seqs, 2 + 2 * seqs]))
+    # plain views of an integer buffer (without the book-keeping of split(), which costs as much as the kernel)
+    return StepPlan(*torch.unsafe_split_with_sizes(out, [cap, cap, cap, cap, seqs, seqs, 2 + 2 * seqs]))
 
 
 class PagedState:
