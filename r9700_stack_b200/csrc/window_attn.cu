@@ -248,10 +248,10 @@ R9K_DEVINL float amax16(const uint4 (&r)[2]) {
 }
 
 // Probabilities are exp2(s - m_ref + P_SHIFT): m_ref follows the running maximum once that has grown by
-// P_LAG (O is rescaled then), so the largest lies in [2^6.5, 2^8.75], below e4m3's 448. Below 2^-6 the
+// P_LAG (O is rescaled then), so the largest lies in [2^6, 2^8.75], below e4m3's 448. Below 2^-6 the
 // first number has steps of 2^-9; the rest, 2^-10 at most, is held to 2^-13 (e5m2) or 2^-14, which is
 // 2^-19 of the largest or less.
-constexpr float P_SHIFT = 6.5f, P_LAG = 2.25f;
+constexpr float P_SHIFT = 6.f, P_LAG = 2.75f;
 
 // One value row (key r of a tile, column halves [H0, H1)) whose key some of the rows do not see. A NaN code
 // in it would reach those rows too (0 * NaN), so such a row of values is cleared, and the rows that do
@@ -727,8 +727,9 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
 // written over the scores in TMEM: as the A operand of PV they cost no shared memory bandwidth, which is
 // what two products on one K or V tile run into (both planes' MMAs read it). MMAs run in order, so S(j + 2)
 // does not overtake PV(j) on the buffer they share, and only a rescale of O has to wait for PV(j - 1).
-// Heads of 128 leave TMEM and shared memory for two CTAs an SM, with one S buffer each: the other CTA's
-// tile fills the gaps, start-up and output included (single CTA, two buffers: see the figures below).
+// One CTA an SM. Two of them with one S buffer each, for which heads of 128 leave room, took 160 us where
+// this takes 146 (3850 ragged tokens, 32 / 8 heads, window 1024): their registers held half the scores, so
+// every score was read and masked twice.
 // K and V tiles share a ring of slots in the order of use, as above. Few tiles: a cluster of CTAs
 // shares the keys of a tile and joins the partial results through distributed shared memory.
 // ------------------------------------------------------------------------------------------------
@@ -741,9 +742,7 @@ template <int D>
 struct Cfg {
   static constexpr int HALVES = D / 128;
   static constexpr int UNIT = KT * D;
-  static constexpr int CTAS = D == 256 ? 1 : 2;   // on an SM
-  static constexpr int SBUF = D == 256 ? 2 : 1;
-  static constexpr int SLOTS = D == 256 ? 5 : 4;
+  static constexpr int SLOTS = D == 256 ? 5 : 8;
   static constexpr int PLANE_Q = ROWS * D;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_RING = OFF_Q + 2 * PLANE_Q;
@@ -753,19 +752,19 @@ struct Cfg {
   static constexpr int NBAR = 1 + 2 * SLOTS + 4;  // q_full, full[], empty[], s_full[2], p_full, pv_done
   static constexpr int OFF_TMEM = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_TMEM + 16;
-  static constexpr int TMEM_COLS = 512 / CTAS;
+  static constexpr int TMEM_COLS = 512;
   static constexpr int O_COL = 0, S_COL = D;  // S buffers of 128 columns; P planes at columns 0 and 32 of them
-  static_assert(D + SBUF * KT <= TMEM_COLS && CTAS * (SMEM + 1024) <= 233472, "TMEM and shared memory");
+  static_assert(D + 2 * KT <= TMEM_COLS && SMEM <= 232448, "TMEM and shared memory");
   static_assert(SLOTS * UNIT >= ROWS * D * 4, "the ring holds the partial results");
 };
 }  // namespace wc
 
 template <int D>
-__global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
+__global__ void __launch_bounds__(wc::THREADS, 1)
     window_attn_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const wa::Args a) {
   using namespace wc;
   using C = Cfg<D>;
-  constexpr int O_COL = C::O_COL, S_COL = C::S_COL, SBUF = C::SBUF;
+  constexpr int O_COL = C::O_COL, S_COL = C::S_COL;
   pdl_wait();
   pdl_trigger();
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -872,16 +871,16 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = *tmem_holder;
-  // the order of use: K0 K1 V0 K2 V1 ... with two S buffers, K0 V0 K1 V1 ... with one
-  auto unit_k = [&](int j) { return SBUF == 1 ? 2 * j : j == 0 ? 0 : 2 * j - 1; };
-  auto unit_v = [&](int j) { return SBUF == 1 ? 2 * j + 1 : j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
+  // the order of use: K0 K1 V0 K2 V1 ...
+  auto unit_k = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
+  auto unit_v = [&](int j) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
 
   if (warp == 0) {
     const bool go = elect_one();
     Pages pages;
     for (int u = 0; u < 2 * n; ++u) {
-        const bool is_k = SBUF == 1 ? !(u & 1) : u == 0 || ((u & 1) && u < 2 * n - 1);
-        const int j = SBUF == 1 ? u / 2 : is_k ? (u + 1) / 2 : u == 2 * n - 1 ? n - 1 : u / 2 - 1;
+        const bool is_k = u == 0 || ((u & 1) && u < 2 * n - 1);
+        const int j = is_k ? (u + 1) / 2 : u == 2 * n - 1 ? n - 1 : u / 2 - 1;
         const int s = u % C::SLOTS;
         if (!warp_wait(&empty[s], (uint32_t)(((u / C::SLOTS) & 1) ^ 1), a.timeout_ns)) {
           if (go) report_error(a.status, kErrMbarTimeout, 322, u);
@@ -907,7 +906,7 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
         if (!wait_unit(u)) return false;
         tc_fence_after();
         const uint64_t kd = k_desc + (uint64_t)((u % C::SLOTS) * (C::UNIT >> 4));
-        const uint32_t d = tbase + S_COL + (j % SBUF) * KT;
+        const uint32_t d = tbase + S_COL + (j & 1) * KT;
 #pragma unroll
         for (int h = 0; h < C::HALVES; ++h)
 #pragma unroll
@@ -916,19 +915,19 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
             for (int pl = 0; pl < 2; ++pl)
               mma_ss(d, q_desc + ((pl * C::PLANE_Q + h * (ROWS * 128) + 32 * k) >> 4), kd + ((h * (KT * 128) + 32 * k) >> 4),
                      idesc_s, h > 0 || k > 0 || pl > 0, go);
-        commit(&s_full[j % SBUF], go);
+        commit(&s_full[j & 1], go);
         commit(&empty[u % C::SLOTS], go);
         return true;
       };
       if (ok) ok = issue_s(0);
       for (int j = 0; ok && j < n; ++j) {
-        if (SBUF == 2 && j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
+        if (j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
         const int u = unit_v(j);
         if (!warp_wait(p_full, (uint32_t)(j & 1), a.timeout_ns)) { ok = false; break; }
         if (!wait_unit(u)) { ok = false; break; }
         tc_fence_after();
         const uint64_t vd = v_desc + (uint64_t)((u % C::SLOTS) * (C::UNIT >> 4));
-        const uint32_t p = tbase + S_COL + (j % SBUF) * KT;
+        const uint32_t p = tbase + S_COL + (j & 1) * KT;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -936,7 +935,6 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
             mma_ts(tbase + O_COL, p + pl * 32 + 8 * k, vd + (k * 4096 >> 4), pl == 0 ? idesc_o[0] : idesc_o[1], j > 0 || k > 0 || pl > 0, go);
         commit(pv_done, go);
         commit(&empty[u % C::SLOTS], go);
-        if (SBUF == 1 && j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
       }
       if (!ok && lane == 0) report_error(a.status, kErrMbarTimeout, 323, 0);
     }
@@ -976,37 +974,28 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
     // A wait that runs out is told to the other warp of the pair (a NaN in place of the maximum, which
     // never is one): both leave at the next exchange, so neither is left at their barrier.
     for (int j = 0; j < n; ++j) {
-      const int s = j % SBUF;
-      ok &= warp_wait(&s_full[s], (uint32_t)((j / SBUF) & 1), a.timeout_ns);
+      const int s = j & 1;
+      ok &= warp_wait(&s_full[s], (uint32_t)((j >> 1) & 1), a.timeout_ns);
       tc_fence_after();
-      // One CTA an SM keeps its 64 scores in registers; two have registers for 32, and read them twice.
-      constexpr int PART = C::CTAS == 1 ? HK : HK / 2;
       const uint32_t scol = trow + S_COL + s * KT + half * HK;
       const int key0 = sp.key(2 * (j0 + j) + half);  // of this thread's page
       const bool whole = whole_page(a, key0, ctx_min, ctx_max);
       // columns that this row sees: [first, first + count), and those before sink
       const int first = max(seen - key0, 0), sink = min(a.sinks, ctx) - key0;
       const uint32_t count = (uint32_t)max(min(ctx - key0, HK) - first, 0);
-      float sv[PART];
-      auto load = [&](int part) {
+      float sv[HK];
 #pragma unroll
-        for (int c = 0; c < PART; c += 16) tmem_ld16(scol + part * PART + c, sv + c);
-        tmem_ld_wait();
-        if (!whole) {
+      for (int c = 0; c < HK; c += 16) tmem_ld16(scol + c, sv + c);
+      tmem_ld_wait();
+      if (!whole) {
 #pragma unroll
-          for (int c = 0; c < PART; ++c)
-            if ((uint32_t)(part * PART + c - first) >= count && part * PART + c >= sink) sv[c] = -INFINITY;
-        }
-      };
-      float tmax = -INFINITY;
-#pragma unroll
-      for (int part = 0; part < HK / PART; ++part) {
-        load(part);
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < PART; ++c) m4[c & 3] = fmaxf(m4[c & 3], sv[c]);
-        tmax = fmaxf(tmax, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        for (int c = 0; c < HK; ++c)
+          if ((uint32_t)(c - first) >= count && c >= sink) sv[c] = -INFINITY;
       }
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < HK; ++c) m4[c & 3] = fmaxf(m4[c & 3], sv[c]);
+      float tmax = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       // value rows of pages that some row does not see whole: a thread a row and column half
       const int vkey = sp.key(2 * (j0 + j) + (q >> 1));
       if (half < C::HALVES && !whole_page(a, vkey, ctx_min, ctx_max)) {
@@ -1034,33 +1023,28 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
       float ls[2] = {0.f, 0.f};
       float ph[HK / 4], pl[HK / 4];  // four 8-bit numbers each
 #pragma unroll
-      for (int part = 0; part < HK / PART; ++part) {
-        if (PART < HK) load(part);
+      for (int c = 0; c < HK; c += 4) {
+        float p[4];
 #pragma unroll
-        for (int c = 0; c < PART; c += 4) {
-          float p[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(sv[c + k], sl2, off));
-          ls[0] += p[0] + p[1];
-          ls[1] += p[2] + p[3];
-          uint32_t h0, l0, h1, l1;
-          split2p<true>(p[0], p[1], h0, l0);
-          split2p<true>(p[2], p[3], h1, l1);
-          ph[(part * PART + c) / 4] = __uint_as_float(h0 | (h1 << 16));
-          pl[(part * PART + c) / 4] = __uint_as_float(l0 | (l1 << 16));
-        }
+        for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(sv[c + k], sl2, off));
+        ls[0] += p[0] + p[1];
+        ls[1] += p[2] + p[3];
+        uint32_t h0, l0, h1, l1;
+        split2p<true>(p[0], p[1], h0, l0);
+        split2p<true>(p[2], p[3], h1, l1);
+        ph[c / 4] = __uint_as_float(h0 | (h1 << 16));
+        pl[c / 4] = __uint_as_float(l0 | (l1 << 16));
       }
       l = l * f + (ls[0] + ls[1]);
-      if (PART < HK) pair_bar();  // the other thread of the row has read its scores again
       // both threads of the row have read their scores (the exchange came after)
       const uint32_t pcol = trow + S_COL + s * KT + half * (HK / 4);
       tmem_st16(pcol, ph);
       tmem_st16(pcol + 32, pl);
       if (__any_sync(0xffffffffu, need)) {
-        // S(j) came after PV(j - SBUF): with two S buffers this product may not be done
-        if (SBUF == 2 && j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
+        // S(j) came after PV(j - 2): this product is the only one that may not be done
+        if (j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
         tc_fence_after();
-#pragma unroll (C::CTAS == 1 ? 2 : 1)
+#pragma unroll 2
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
           float o[32];
           tmem_ld16(trow + O_COL + c, o);
@@ -1075,7 +1059,7 @@ __global__ void __launch_bounds__(wc::THREADS, wc::Cfg<D>::CTAS)
       tmem_st_wait();
       // A parity tells neighbouring phases apart only. The wait after the loop is for the last product, so the
       // one before it is waited for here, where the last cannot have run yet.
-      if (SBUF == 2 && j == n - 1 && j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
+      if (j == n - 1 && j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
       tc_fence_before();
       mbar_arrive(p_full);
     }
@@ -1294,7 +1278,7 @@ void window_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
   const int64_t groups = dec ? S : std::min(T / per + S, S * ((a.max_new + per - 1) / per));
   // CTAs of a cluster share a group's keys while that fills the GPU and leaves each of them a tile
   int64_t nsplit = 1;
-  while (nsplit < 8 && groups * Hkv * nsplit * 2 <= sms * (dec || D == 128 ? 2 : 1) && nsplit * 2 <= tiles) nsplit *= 2;
+  while (nsplit < 8 && groups * Hkv * nsplit * 2 <= sms * (dec ? 2 : 1) && nsplit * 2 <= tiles) nsplit *= 2;
   const dim3 grid((unsigned)groups, (unsigned)Hkv, (unsigned)nsplit);
   TORCH_CHECK(groups <= INT_MAX, "window_attention: too many rows");
   if (dec) {
