@@ -842,6 +842,11 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
       qraw[c][1] = src[1];
     }
   }
+  if (valid && a.gate != nullptr && nsplit == 1) {  // wanted at the end: from DRAM to L2 meanwhile
+    const char* g = reinterpret_cast<const char*>(a.gate + (int64_t)tok * a.ld_gate + head * D + half * (D / 2));
+#pragma unroll
+    for (int i = 0; i < D; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + i));
+  }
   const int ctx = valid ? context(a, tok) : 0;
   int ctx_min, ctx_max;
   context_range(a, tok0, ntok, ctx_min, ctx_max);
