@@ -10,8 +10,7 @@
 // one (finer than the 2^-24 steps of the uniform number itself), so every sum is exact: the token
 // depends on the row and its number alone, not on the order of additions, the batch or the launch.
 //
-// A row belongs to a cluster of CTAs; each holds a slice of it in shared memory, so the logits are read
-// from memory once. Both cuts look for "the smallest key B with F(keys <= B) >= target", F = count or
+// A row belongs to a cluster of CTAs; each has a slice of it, held in shared memory or read again from L2. Both cuts look for "the smallest key B with F(keys <= B) >= target", F = count or
 // weight, keys ordered as above:
 //   * a histogram of (m - x) / T over 1024 bins a CTA (shared-memory atomics on whole numbers), summed by
 //     the cluster's first CTA, gives the bin in which F crosses the target. Top-k first tries the
@@ -22,6 +21,11 @@
 //   * else the crossing bin's keys are sorted there (after a second, 1024 times finer histogram if they
 //     are many; bit by bit over the cluster if thousands tie), and the cut key goes back to all CTAs,
 //     which sum and draw over their slices.
+//
+// What bounds it: for few rows the chain of exchanges (a cluster barrier and a remote read are about 1 us
+// each; one row of 248320 fp32: 13.8 us, of which 3 us load it); for many rows the second read and the
+// exchanges of rows that share an SM (256 rows: 120 us, the first read alone 39 us at copy bandwidth); for
+// wide nuclei the histogram's three atomics a key (64 x 100003 bf16: 54 us).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -423,7 +427,7 @@ R9K_DEVINL void finish_list(const Args& a, const Row& r, int row, int n, u64 all
 
 // HELD: the slice is kept in shared memory as fp32; else it is read again (from L2) by each pass
 template <typename T, bool HELD>
-__global__ void __launch_bounds__(sm::THREADS, HELD ? 2 : 3) sample_kernel(const sm::Args a) {
+__global__ void __launch_bounds__(sm::THREADS, 2) sample_kernel(const sm::Args a) {
   using namespace sm;
   using U = std::conditional_t<HELD, float, T>;
   pdl_wait();
@@ -734,19 +738,20 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   TORCH_CHECK(V <= (int64_t)sm::MAX_CLUSTER * MAX_SLICE, "sample_logits: vocabulary too large");
   if (R == 0) return;
   const at::cuda::CUDAGuard guard(logits.device());
-  // The most CTAs a row that still let all rows run in one wave, a slice of at least 4096; where no count does,
-  // the fewest. A wave is three CTAs an SM for slices read twice, two for held ones (below), and clusters leave
-  // some of it unused. Measured, CTAs a row x 16 / 8 / 4: 256 rows x 248320 fp32, top-k, 250 / 158 / 124 us; 64
-  // rows 84 / 61 / -; 16 rows 35 / 30 / -; 64 rows x 100003 bf16, top-p, 86 / 59 / 54 us.
+  // The most CTAs a row that still let all rows run in one wave (two CTAs an SM, of which clusters leave an
+  // eighth, those of 16 a quarter unused), a slice of at least 4096; where no count does, the fewest. Measured,
+  // CTAs a row x 16 / 8 / 4: 256 rows x 248320 fp32, top-k, 250 / 158 / 120 us; 64 rows 84 / 61 / -; 16 rows
+  // 35 / 28 / -; 64 rows x 100003 bf16, top-p, 86 / 59 / 54 us.
   const int64_t sms = device_sm_count();
   auto slice_of = [&](int c) { return ((V + c - 1) / c + 3) / 4 * 4; };
+  auto wave = [&](int c) { return c == 16 ? sms * 3 / 2 : sms * 7 / 4; };
   int least = 1;
   while (slice_of(least) > 65532) least *= 2;
   int C = sm::MAX_CLUSTER;
-  while (C > least && (slice_of(C) < 4096 || R * C > (C == 16 ? sms * 3 / 2 : sms * 5 / 2))) C /= 2;
-  // Slices held in shared memory are read once, but leave room for two CTAs an SM: while that wave takes
-  // all rows too (64 x 100003 bf16, 4 CTAs a row: 54 us held, 68 not; one row, 16 CTAs: 13.7 held, 15.4 not).
-  const bool held = slice_of(C) <= HELD_SLICE && R * C <= (C == 16 ? sms * 3 / 2 : sms * 7 / 4);
+  while (C > least && (slice_of(C) < 4096 || R * C > wave(C))) C /= 2;
+  // Slices held in shared memory are read once; as long as two of them fit an SM and one wave takes all rows
+  // (64 x 100003 bf16, 4 CTAs a row: 54 us held, 68 not; one row, 16 CTAs: 13.7 held, 15.4 not).
+  const bool held = slice_of(C) <= HELD_SLICE && R * C <= wave(C);
   TORCH_CHECK(R * C <= INT_MAX, "sample_logits: too many rows");
   sm::Args a{logits.data_ptr(), logits.stride(0), (int)V, (int)slice_of(C), u.data_ptr<float>(),
              temperature.data_ptr<float>(), top_k.has_value() ? top_k->data_ptr<int32_t>() : nullptr,
