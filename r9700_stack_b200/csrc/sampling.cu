@@ -715,6 +715,20 @@ __global__ void __launch_bounds__(sm::THREADS, 2) sample_kernel(const sm::Args a
   }
 }
 
+// Clusters of 16 have to be asked for, once a kernel and device.
+static cudaError_t allow_wide_clusters(const void* kern) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lk(mu);
+  if (done.count({kern, dev})) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.insert({kern, dev});
+  return e;
+}
+
 void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperature, c10::optional<torch::Tensor> top_k,
                    c10::optional<torch::Tensor> top_p, c10::optional<torch::Tensor> min_p, torch::Tensor tokens,
                    torch::Tensor logprobs) {
@@ -762,8 +776,7 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   auto kern = held ? (f32 ? sample_kernel<float, true> : sample_kernel<__nv_bfloat16, true>)
                    : (f32 ? sample_kernel<float, false> : sample_kernel<__nv_bfloat16, false>);
   TORCH_CHECK(ensure_smem_attr((const void*)kern, sm::WORK_BYTES + (held ? HELD_SLICE * 4 + 16 : 0)) == cudaSuccess &&
-                  cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess,
-              "sample_logits: kernel attributes");
+                  allow_wide_clusters((const void*)kern) == cudaSuccess, "sample_logits: kernel attributes");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(R * C));
   cfg.blockDim = dim3(sm::THREADS);

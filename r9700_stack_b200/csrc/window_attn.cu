@@ -331,7 +331,6 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
   using C = Cfg<D, NC>;
   constexpr int N = C::N, S_COL = C::S_COL, O_COL = C::O_COL;
   pdl_wait();
-  pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -392,6 +391,9 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Only now: a dependent kernel that takes TMEM ahead of its own wait must not come between a CTA of this
+  // grid and its columns.
+  pdl_trigger();
   const uint32_t tbase = *tmem_holder;
   // the order of use: K0, then K(j + 1) (if there is one) and V(j)
   auto unit_v = [&](int j) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; };
@@ -780,7 +782,6 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
   using C = Cfg<D>;
   constexpr int O_COL = C::O_COL, S_COL = C::S_COL;
   pdl_wait();
-  pdl_trigger();
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_full = bars;
@@ -828,6 +829,16 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
       }
       before += __shfl_sync(0xffffffffu, inc, 31);
     }
+  }
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && split == 0 && warp == 0) {
+    // the grid holds the tiles of T tokens: sequences that share tokens would need more
+    int all = 0;
+    for (int i = lane; i < a.S; i += 32) {
+      const int len = a.seq_len[i];
+      if (len > 0 && len <= a.max_new) all += (len + per - 1) / per;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (all > (int)gridDim.x && lane == 0) report_error(a.status, kErrBounds, 326, all);
   }
   if (seq < 0) return;  // the grid is a bound: the same in the whole cluster
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it
@@ -889,6 +900,9 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Only now: a dependent kernel that takes TMEM ahead of its own wait must not come between a CTA of this
+  // grid and its columns.
+  pdl_trigger();
   const uint32_t tbase = *tmem_holder;
   // the order of use: K0 K1 V0 K2 V1 ...
   auto unit_k = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };

@@ -16,7 +16,7 @@ import math
 
 import torch
 
-from ..models.hybrid import StepMeta
+from ..models.hybrid import HybridLM, StepMeta
 from ..ops.sampling import sample_tokens
 from ..ops.step_plan import PAGE, PagedState, plan_numel
 from ..utils import status as _status
@@ -26,6 +26,8 @@ from .scheduler import SamplingParams
 
 class DeviceLoop:
     def __init__(self, model, seqs: int, max_len: int, max_prefill_tokens: int = 2048):
+        if not isinstance(model, HybridLM) or model.comm.world_size > 1:
+            raise ValueError("DeviceLoop: a hybrid model on one GPU")
         c = model.cfg
         if seqs < 1 or max_len < 2 or max_prefill_tokens < 1:
             raise ValueError("need at least one sequence, two tokens and one prefill token")
@@ -124,7 +126,8 @@ class DeviceLoop:
 
     def decode(self, steps: int):
         """Draw ``steps`` more tokens for every sequence; returns (tokens [steps, seqs] int64, logprobs), on
-        the device and not waited for. The last drawn token has not been run yet, as in ``LLM``."""
+        the device and not waited for (``utils.status.check`` tells afterwards whether a device wait failed). The
+        last drawn token has not been run yet, as in ``LLM``."""
         if not self.ctx:
             raise RuntimeError("DeviceLoop: prefill() first")
         if steps < 1 or max(self.ctx) + steps > self.max_len:

@@ -99,6 +99,8 @@ def test_loop_refusals():
     for bad in ((0, 64, 8), (1, 1, 8), (1, 64, 0)):
         with pytest.raises(ValueError):
             DeviceLoop(model, *bad)
+    with pytest.raises(ValueError):
+        DeviceLoop(object(), 1, 64, 8)
     loop = DeviceLoop(model, 2, 64, 16)
     with pytest.raises(RuntimeError):
         loop.decode(1)

@@ -252,6 +252,12 @@ def test_refusals():
     torch.cuda.synchronize()
     with pytest.raises(status.DeviceWaitError):
         status.check()
+    two = _case([70, 10], [60, 60], 8, 2, 128, seed=4)
+    two["seq_start"][1], two["seq_len"][:] = 0, 120  # both claim every token
+    window_attention(**two)
+    torch.cuda.synchronize()
+    with pytest.raises(status.DeviceWaitError):
+        status.check()
     c["block_table"][0, 0] = 10**6
     window_attention(**c)
     torch.cuda.synchronize()
