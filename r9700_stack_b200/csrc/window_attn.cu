@@ -741,11 +741,12 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
 // K and V tiles share a ring of slots in the order of use, as above. Few tiles: a cluster of CTAs
 // shares the keys of a tile and joins the partial results through distributed shared memory.
 //
-// What bounds it: 8192 tokens, 24 / 4 heads of 256, window 4096: 890 us, 927 TFLOP/s of useful products, 0.55
-// of the bf16 rate (the tensor pipe is busy 0.46 of the time at the 8-bit rate, on two planes). A key tile
-// takes about 2900 cycles: 2050 of MMA at the least, beside a softmax of about 2200 (two exponentials a
-// cycle and SM sub-partition are 1024 of them) whose scores, maxima and probabilities follow one another.
-// Ragged prompts, 3850 tokens, 32 / 8 heads of 128, window 1024: 145 us; ten key tiles a CTA do not hide
+// What bounds it: 8192 tokens, 24 / 4 heads of 256, window 4096: 890 to 975 us with the card's clocks, 850 to
+// 930 TFLOP/s of useful products, 0.51 to 0.55 of the bf16 rate (the tensor pipe is busy 0.46 of the time at the
+// 8-bit rate, on two planes). A key tile takes about 2900 cycles: 2050 of MMA at the least, beside a softmax of
+// about 2200 (1024 of them the exponential unit's 16 a cycle) whose scores, maxima and probabilities follow one
+// another.
+// Ragged prompts, 3850 tokens, 32 / 8 heads of 128, window 1024: 147 us; ten key tiles a CTA do not hide
 // its start (page and length reads, queries) and end, 13000 cycles together.
 // Shares of 1 / 2 / 4 / 8 CTAs for 16 sequences x 1..8 drafts, 16 / 2 heads: 34 / 27 / 21 / 44 us.
 // ------------------------------------------------------------------------------------------------

@@ -20,10 +20,10 @@ class SamplingParams:
     temperature: float = 0.0
     top_k: int = 0
     top_p: float = 1.0
-    min_p: float = 0.0  # tokens less likely than min_p times the likeliest are dropped (0: off)
     ignore_eos: bool = True
     eos_token_id: int = -1
     seed: int = 0
+    min_p: float = 0.0  # tokens less likely than min_p times the likeliest are dropped (0: off)
 
 
 _ids = itertools.count()
