@@ -188,8 +188,7 @@ def _prepare_sample(case, seed):
     # a vocabulary's bulk, and a few tokens that the context favours, more or less clearly
     x = torch.randn(rows, vocab, generator=g, device="cuda") * 2.0
     few = min(40, vocab)
-    # (places of one row differ: a place written twice would hold whichever write came last)
-    at = (torch.randint(0, vocab, (rows, 1), generator=g, device="cuda") + torch.arange(few, device="cuda") * (vocab // few)) % vocab
+    at = torch.randint(0, vocab, (rows, few), generator=g, device="cuda")
     lift = torch.rand(rows, few, generator=g, device="cuda") * 8 + torch.rand(rows, 1, generator=g, device="cuda") * 8
     x.scatter_(1, at, lift + 4)
     f = lambda a: torch.from_numpy(a.astype(np.float32)).cuda()  # noqa: E731
