@@ -766,7 +766,7 @@ struct Cfg {
   static constexpr int OFF_RED = OFF_RING + SLOTS * UNIT;  // maxima [parity][half][ROWS]; at the end l[half][ROWS], m[ROWS]
   static constexpr int OFF_POISON = OFF_RED + 4 * ROWS * 4;  // bytes by token
   static constexpr int OFF_BAR = OFF_POISON + ROWS;
-  static constexpr int NBAR = 1 + 2 * SLOTS + 4;  // q_full, full[], empty[], s_full[2], p_full, pv_done
+  static constexpr int NBAR = 1 + 2 * SLOTS + 6;  // q_full, full[], empty[], s_full[2], p_full[2], pv_done[2]
   static constexpr int OFF_TMEM = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_TMEM + 16;
   static constexpr int TMEM_COLS = 512;
@@ -790,7 +790,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
   uint64_t* empty = full + C::SLOTS;
   uint64_t* s_full = empty + C::SLOTS;
   uint64_t* p_full = s_full + 2;
-  uint64_t* pv_done = p_full + 1;
+  uint64_t* pv_done = p_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_TMEM);
   float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
   float* row_l = red;             // [half][ROWS]
@@ -886,9 +886,11 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) mbar_init(&s_full[s], 1);
-    mbar_init(p_full, SOFT);
-    mbar_init(pv_done, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], SOFT);
+      mbar_init(&pv_done[s], 1);
+    }
     fence_mbar_init();
     prefetch_tmap(&tmK);
     prefetch_tmap(&tmV);
@@ -957,7 +959,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
       for (int j = 0; ok && j < n; ++j) {
         if (j + 1 < n && !issue_s(j + 1)) { ok = false; break; }
         const int u = unit_v(j);
-        if (!warp_wait(p_full, (uint32_t)(j & 1), a.timeout_ns)) { ok = false; break; }
+        if (!warp_wait(&p_full[j & 1], (uint32_t)((j >> 1) & 1), a.timeout_ns)) { ok = false; break; }
         if (!wait_unit(u)) { ok = false; break; }
         tc_fence_after();
         const uint64_t vd = v_desc + (uint64_t)((u % C::SLOTS) * (C::UNIT >> 4));
@@ -967,7 +969,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
 #pragma unroll
           for (int pl = 0; pl < 2; ++pl)
             mma_ts(tbase + O_COL, p + pl * 32 + 8 * k, vd + (k * 4096 >> 4), pl == 0 ? idesc_o[0] : idesc_o[1], j > 0 || k > 0 || pl > 0, go);
-        commit(pv_done, go);
+        commit(&pv_done[j & 1], go);
         commit(&empty[u % C::SLOTS], go);
       }
       if (!ok && lane == 0) report_error(a.status, kErrMbarTimeout, 323, 0);
@@ -1074,9 +1076,11 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
       const uint32_t pcol = trow + S_COL + s * KT + half * (HK / 4);
       tmem_st16(pcol, ph);
       tmem_st16(pcol + 32, pl);
+      // A parity tells neighbouring phases apart only, so every phase of a barrier is looked at, here or in the
+      // MMA warp, before the next but one can complete. PV(j - 2) is done (S(j) came after it): this never waits long.
+      if (j >= 2) ok &= warp_wait(&pv_done[s], (uint32_t)(((j - 2) >> 1) & 1), a.timeout_ns);
       if (__any_sync(0xffffffffu, need)) {
-        // S(j) came after PV(j - 2): this product is the only one that may not be done
-        if (j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
+        if (j > 0) ok &= warp_wait(&pv_done[(j - 1) & 1], (uint32_t)(((j - 1) >> 1) & 1), a.timeout_ns);
         tc_fence_after();
 #pragma unroll 2
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
@@ -1091,11 +1095,8 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
         }
       }
       tmem_st_wait();
-      // A parity tells neighbouring phases apart only. The wait after the loop is for the last product, so the
-      // one before it is waited for here, where the last cannot have run yet.
-      if (j == n - 1 && j > 0) ok &= warp_wait(pv_done, (uint32_t)((j - 1) & 1), a.timeout_ns);
       tc_fence_before();
-      mbar_arrive(p_full);
+      mbar_arrive(&p_full[s]);
     }
     uint4 graw[QC][2] = {};  // the gate of this thread's half of the output, on its way during the last product
     if (nsplit == 1 && valid && a.gate != nullptr) {
@@ -1106,7 +1107,7 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
         graw[c][1] = g[2 * c + 1];
       }
     }
-    if (n > 0 && ok) ok = warp_wait(pv_done, (uint32_t)((n - 1) & 1), a.timeout_ns);
+    if (n > 0 && ok) ok = warp_wait(&pv_done[(n - 1) & 1], (uint32_t)(((n - 1) >> 1) & 1), a.timeout_ns);
     tc_fence_after();
     if (!ok) report_error(a.status, kErrMbarTimeout, 324, r);
     const bool have = n > 0 && ok;
