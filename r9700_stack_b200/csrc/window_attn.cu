@@ -68,7 +68,7 @@ R9K_DEVINL Span make_span(const Args& a, int ctx_min, int ctx_max) {
   return s;
 }
 
-// whether every row (contexts in [ctx_min, ctx_max]) sees the whole page at key
+// whether every row that sees anything (contexts in [ctx_min, ctx_max]) sees the whole page at key
 R9K_DEVINL bool whole_page(const Args& a, int key, int ctx_min, int ctx_max) {
   return key + PAGE <= ctx_min && (a.window == 0 || key >= ctx_max - a.window || key + PAGE <= a.sinks);
 }
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
     const int q = warp & 3;
     const int r = q * 32 + lane;      // TMEM lane: key of the tile, then dim of the output
     const int tr = threadIdx.x - 64;  // 0..127
-    // columns past NQ: a zero query and context 0, so every key is masked; eight threads a query row
+    // columns past NQ: a zero query and context 0, which gives them no weight at the end; eight threads a query row
     {
       const int row = tr >> 3, part = tr & 7;
       const bool valid = row < NQ;
@@ -657,6 +657,7 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
         col_m[c] = n > 0 && ok ? mref[c] : -INFINITY;
         col_l[c] = n > 0 && ok ? (l4.x + l4.y) + (l4.z + l4.w) : 0.f;
         if (c < NQ && poison[c / a.G]) col_l[c] = __int_as_float(0x7fffffff);
+        if (col_ctx[c] == 0) col_l[c] = 0.f;  // sees nothing (its scores of whole pages were not masked)
       }
   }
   __syncwarp();  // the cluster's barrier wants whole warps

@@ -153,6 +153,29 @@ def test_rows_that_see_nothing_and_uncovered_rows(new):
     assert bool((got[new[0]: new[0] + new[1]] == 5.0).all())
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(12, 4, 256), (16, 8, 128), (12, 4, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 4)])
+def test_a_row_without_context_beside_rows_with_many_keys(hq, hkv, d, window, sinks):
+    """Context 0 gives a zero row also where the other tokens of its sequence see whole pages, NaN values in them or
+    not; the other rows are those of a sequence without it."""
+    c = _case([500, 300, 129], [5, 3, 4], hq, hkv, d, seed=15, gate=False)
+    want = _run(c, window, sinks, max_new=5)
+    dead = [2, 5, 11]
+    live = [t for t in range(12) if t not in dead]
+    for t in dead:
+        c["tok_ctx"][t] = 0
+    out = _run(c, window, sinks, max_new=5)
+    assert bool((out[dead] == 0).all())
+    ref, tol = _bound(c, window, sinks)
+    assert bool(((out.double() - ref).abs() <= tol).all())
+    assert torch.equal(out[live], want[live])
+    for key in (460, 400):  # in a page of which the rows see a part, and in one that they see whole
+        page = int(c["block_table"][0, key // PAGE])
+        c["v_cache"][page, :, key % PAGE, 3] = 0x7F
+        out = _run(c, window, sinks, max_new=5)
+        assert bool((out[dead] == 0).all()) and torch.equal(out[live][4:], want[live][4:])
+
+
 @pytest.mark.parametrize("new", [1, 6, 90])
 def test_hidden_keys_do_not_matter(new):
     """Positions past the context, pages that left the window and unused table entries may hold
