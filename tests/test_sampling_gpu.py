@@ -177,6 +177,63 @@ def test_degenerate_rows(V):
         assert int(tok[2]) == 17 and 0 <= int(tok[9]) < V
 
 
+def _check_batch(x, u, par, some):
+    """All rows of a wide batch, whose slices are read again instead of being held in shared memory: the
+    tokens and log-probabilities that a few rows at a time give (their slices are held), and, of the rows ``some``, the
+    definition's."""
+    from r9700_stack_b200.ops.sampling import sample_tokens
+
+    tok, lp = sample_tokens(x, u, *par)
+    cut = lambda v, at: None if v is None else v[at]  # noqa: E731
+    for i in range(0, x.shape[0], 8):
+        at = slice(i, i + 8)
+        t, l = sample_tokens(x[at], u[at], *[cut(v, at) for v in par])
+        assert torch.equal(tok[at], t) and torch.equal(lp[at], l)
+    at = torch.tensor(some, device="cuda")
+    rows = torch.stack([x[i] for i in some])
+    t, l = _check(rows, u[at], *[cut(v, at) for v in par])
+    assert torch.equal(tok[at], t) and torch.equal(lp[at], l)
+    return tok
+
+
+@pytest.mark.parametrize("kind", ["plain", "k", "p", "m", "all", "greedy", "hot", "cold", "wide k"])
+@pytest.mark.parametrize("R,V,dtype,ld", [(300, 20011, torch.float32, 20011), (300, 20011, torch.bfloat16, 20013),
+                                          (70, 90001, torch.float32, 90003), (130, 60002, torch.bfloat16, 60007),
+                                          (66, 200003, torch.bfloat16, 200009), (260, 140001, torch.float32, 140001)])
+def test_wide_batches_match_the_definition(R, V, dtype, ld, kind):
+    """More rows than run at once: one CTA a row and several, odd sizes, rows that start off the 16-byte grid."""
+    g = torch.Generator(device="cuda").manual_seed(V + len(kind) + R)
+    x = torch.randn(R, ld, generator=g, device="cuda") * 2.5
+    x[:, :: max(1, V // 20)] += 7
+    x = x.to(dtype)[:, ld - V:]
+    u = torch.rand(R, generator=g, device="cuda")
+    u[0], u[1] = 0.0, 0.99999994
+    _check_batch(x, u, _params(R, g, kind), [0, 1, R // 2, R - 1])
+
+
+@pytest.mark.parametrize("R,V", [(300, 20011), (80, 100003)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_wide_batches_of_ties(R, V, dtype):
+    """Thousands of equal logits around the cuts, in one place of the histogram and in all slices."""
+    g = torch.Generator(device="cuda").manual_seed(R)
+    x = torch.randn(R, V, generator=g, device="cuda")
+    x[::3] = 0.0
+    x[1::3, 3::7] = 6.0
+    x[2::3, V // 2: V // 2 + 1500] = 5.0
+    x[R - 1] = -float("inf")
+    x[R - 2] = float("nan")
+    x[R - 3] = torch.finfo(dtype).min
+    x[R - 3, V - 1] = 2.0
+    u = torch.rand(R, generator=g, device="cuda")
+    k = torch.randint(1, 4000, (R,), generator=g, device="cuda", dtype=torch.int32)
+    p = torch.rand(R, generator=g, device="cuda")
+    one = torch.ones(R, device="cuda")
+    for par in ((one, k, None, None), (one, None, p, None), (one * 0.7, k, p, one * 0.01)):
+        tok = _check_batch(x.to(dtype), u, par, [0, 1, 2, R - 3, R - 2, R - 1])
+        assert tok[R - 2:].tolist() == [-1, -1] and int(tok[R - 3]) == V - 1
+        assert bool((tok[0: R - 3: 3] < 4000).all()) or par[1] is None
+
+
 def test_strided_rows_batch_invariance_and_stream():
     from r9700_stack_b200.ops.sampling import sample_tokens
 
