@@ -817,8 +817,6 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
         const int x = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += x;
       }
-      if (blockIdx.x == 0 && blockIdx.y == 0 && split == 0 && warp == 0 && len > a.max_new)
-        report_error(a.status, kErrConfig, 320, len);
       const uint32_t hit = __ballot_sync(0xffffffffu, (int)blockIdx.x < before + inc);
       if (hit != 0) {
         const int src = __ffs((int)hit) - 1;
@@ -833,11 +831,13 @@ __global__ void __launch_bounds__(wc::THREADS, 1)
     }
   }
   if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && split == 0 && warp == 0) {
-    // the grid holds the tiles of T tokens: sequences that share tokens would need more
+    // One warp of the grid looks at every sequence (the search above ends at the block's own). The grid holds the
+    // tiles of T tokens: sequences that share tokens would need more.
     int all = 0;
     for (int i = lane; i < a.S; i += 32) {
       const int len = a.seq_len[i];
-      if (len > 0 && len <= a.max_new) all += (len + per - 1) / per;
+      if (len > a.max_new) report_error(a.status, kErrConfig, 320, len);
+      else if (len > 0) all += (len + per - 1) / per;
     }
     all = __reduce_add_sync(0xffffffffu, all);
     if (all > (int)gridDim.x && lane == 0) report_error(a.status, kErrBounds, 326, all);

@@ -256,6 +256,37 @@ def test_same_inputs_same_bits():
             assert torch.equal(_run(c, 0, 0), a)
 
 
+@pytest.mark.parametrize("most", [1, 5, 20])
+def test_more_sequences_than_a_warp_reads_at_once(most):
+    """77 sequences of 0 to ``most`` tokens: single tokens, drafts, chunks."""
+    g = torch.Generator().manual_seed(most)
+    new = torch.randint(0, most + 1, (77,), generator=g).tolist()
+    new[40], new[76] = most, most
+    ctx = torch.randint(0, 200, (77,), generator=g).tolist()
+    _check(_case(ctx, new, 12, 4, 128, seed=16), 90, 3, max_new=most)
+
+
+@pytest.mark.parametrize("most", [4, 6])
+@pytest.mark.parametrize("at", [3, 35, 76])
+def test_a_sequence_over_its_bound_is_reported_wherever_it_stands(most, at):
+    from r9700_stack_b200.ops.window_attention import window_attention
+    from r9700_stack_b200.utils import status
+
+    new = [most] * 77
+    new[at] = most + 3
+    c = _case([70] * 77, new, 12, 4, 128, seed=17, gate=False)
+    out = torch.full((sum(new), 12 * 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    window_attention(**c, max_new=most, out=out)
+    torch.cuda.synchronize()
+    with pytest.raises(status.DeviceWaitError):
+        status.check()
+    first = most * at
+    assert bool((out[first: first + most + 3] == 5.0).all())
+    ref, tol = _bound(c, 0, 0)
+    others = [t for t in range(sum(new)) if not first <= t < first + most + 3]
+    assert bool(((out.double() - ref).abs() <= tol)[others].all())
+
+
 def test_refusals():
     from r9700_stack_b200.ops.window_attention import window_attention
     from r9700_stack_b200.utils import status
