@@ -65,9 +65,10 @@ def uniform(seed: int, step: int) -> float:
 
 
 def device_params(params_list, device):
-    """(temperature, top_k, top_p, min_p) of one request a row, as ``ops.sampling.sample_tokens`` takes them."""
+    """(temperature, top_k, top_p, min_p) of one request a row, as ``ops.sampling.sample_tokens`` takes them.
+    A top_k that no vocabulary reaches is off, as in :func:`sample_rows` (int32 could not hold every one)."""
     f = lambda name: torch.tensor([float(getattr(p, name)) for p in params_list], dtype=torch.float32, device=device)
-    k = torch.tensor([p.top_k for p in params_list], dtype=torch.int32, device=device)
+    k = torch.tensor([p.top_k if p.top_k and 0 < p.top_k < 2**31 else 0 for p in params_list], dtype=torch.int32, device=device)
     return f("temperature"), k, f("top_p"), f("min_p")
 
 

@@ -33,6 +33,16 @@ def test_device_params():
     assert p.dtype == torch.float32 and abs(float(m[1]) - 0.1) < 1e-7
 
 
+def test_device_params_take_any_top_k():
+    """A number past int32 keeps everything, as in the host sampler; it must not end the step that all requests share."""
+    ks = [2**40, -2**40, 2**31, 2**31 - 1, -1, 0, None, 7]
+    _, k, _, _ = device_params([SamplingParams(temperature=1.0, top_k=v) for v in ks], "cpu")
+    assert k.dtype == torch.int32 and k.tolist() == [0, 0, 0, 2**31 - 1, 0, 0, 0, 7]
+    x = torch.log(torch.tensor([[0.5, 0.3, 0.15, 0.05]])).expand(len(ks), 4)
+    params = [SamplingParams(temperature=1.0, top_k=v, seed=1) for v in ks]
+    assert len(sample_rows(x, params, [0] * len(ks))) == len(ks)
+
+
 def test_sample_ref_on_cpu():
     f = lambda v: torch.tensor(v, dtype=torch.float32)
     x = torch.log(torch.tensor([[0.1, 0.4, 0.2, 0.3]])).expand(5, 4)
