@@ -40,6 +40,7 @@ class DeviceLoop:
         if self.window:
             # sinks, the window, and two chunks: pages go back one step after they left the window
             held = min(width, math.ceil(self.sinks / PAGE) + math.ceil((self.window + 2 * max_prefill_tokens) / PAGE) + 2)
+        model.ensure_positions(max_len)
         dev = self.device = model.device
         self.pages = PagedState(seqs * held + 1, seqs, width, dev)
         model.alloc_caches(seqs * held + 1, seqs + 1, PAGE)

@@ -35,6 +35,7 @@ class LLM:
             model = build_model(model_cfg, self.par, self.device, seed=seed, comm=comm, max_ctx=ec.max_model_len,
                                 placement=placement)
         self.model = model
+        model.ensure_positions(ec.max_model_len + 64)  # as far as the scheduler lets drafts reach
         blocks_per_seq = math.ceil(ec.max_model_len / ec.kv_block)
         num_blocks = ec.num_kv_blocks or (ec.max_batch * blocks_per_seq + 1)
         num_slots = ec.max_batch + 1

@@ -231,6 +231,14 @@ class HybridLM:
         assert len(kinds) == 1, "every layer's linear weights must be MX, or all bf16 / native NVFP4"
         self.mx = kinds.pop()
 
+    outgrown = ()  # rotary tables that were replaced: a graph captured with one goes on reading it
+
+    def ensure_positions(self, n: int) -> None:
+        """Have the rotary table cover positions [0, n): the kernels read it by position, without a bound."""
+        if n > self.cos_sin.shape[0]:
+            self.outgrown = (*self.outgrown, self.cos_sin)
+            self._rope_cache(n)
+
     def _rope_cache(self, max_pos: int):
         c = self.cfg
         rot = c.rotary_dim

@@ -216,6 +216,11 @@ class MLAMoELM:
             n += sum(weight_nbytes(v) for v in lay.values())
         return n
 
+    def ensure_positions(self, n: int) -> None:
+        """Refuse positions past the rotary table (its length, like the workspaces', is the model's ``max_ctx``)."""
+        if n > self.cos_sin.shape[0]:
+            raise ValueError(f"the model is built for contexts of {self.max_ctx} tokens")
+
     def alloc_caches(self, num_kv_blocks: int, num_state_slots: int, kv_block: int = 64):
         assert kv_block == 64
         self.lat, self.icache = {}, {}

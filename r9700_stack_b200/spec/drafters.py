@@ -127,6 +127,7 @@ class ModelDrafter(Drafter):
         self.kind = kind
         self.model = build_draft_model(target_model, kind, seed=seed)
         self.bs = engine_cfg.kv_block
+        self.model.ensure_positions(engine_cfg.max_model_len + 64)
         self.model.alloc_caches(num_blocks, num_slots, engine_cfg.kv_block)
         mb = engine_cfg.max_batch
         self.max_tokens = engine_cfg.max_prefill_tokens + mb * (k + 2)

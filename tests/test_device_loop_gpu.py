@@ -70,6 +70,24 @@ def test_loop_gives_the_engines_tokens():
     assert loop.pages.ctx_len.tolist() == [449]
 
 
+def test_loop_past_the_length_the_model_was_built_for():
+    """The rotary table ends within the prompt; the loop grows it, and a loop captured before keeps its own."""
+    from r9700_stack_b200.engine.device_loop import DeviceLoop
+    from r9700_stack_b200.models.hybrid import HybridLM
+
+    cfg = _cfg()
+    prompt = _prompt(150, cfg.vocab)
+    runs = []
+    for rows in (65536, 100):
+        model = HybridLM(cfg, device="cuda", seed=7)
+        model._rope_cache(rows)
+        loop = DeviceLoop(model, 1, 600, max_prefill_tokens=64)
+        runs.append(loop.prefill([prompt]) + loop.decode(20)[0][:, 0].tolist())
+        model.ensure_positions(100000)
+        runs[-1] += loop.decode(100)[0][:, 0].tolist()
+    assert runs[0] == runs[1]
+
+
 def test_loop_samples_and_repeats():
     from r9700_stack_b200.engine.device_loop import DeviceLoop
     from r9700_stack_b200.engine.scheduler import SamplingParams
