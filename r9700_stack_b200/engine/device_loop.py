@@ -44,6 +44,7 @@ class DeviceLoop:
         dev = self.device = model.device
         self.pages = PagedState(seqs * held + 1, seqs, width, dev)
         model.alloc_caches(seqs * held + 1, seqs + 1, PAGE)
+        self.caches = model.held_caches()
         self.ws = model.alloc_workspace(max(max_prefill_tokens, seqs), seqs)
         i32 = dict(dtype=torch.int32, device=dev)
         self.ids = torch.zeros(seqs, **i32)
@@ -78,6 +79,7 @@ class DeviceLoop:
         params = params or [SamplingParams()] * self.seqs
         if len(params) != self.seqs:
             raise ValueError("one SamplingParams a sequence")
+        self.model.use_caches(self.caches)
         self.params = device_params(params, self.device)
         self.seeds = [p.seed for p in params]
         u0 = torch.tensor([uniform(s, 0) for s in self.seeds], dtype=torch.float32, device=self.device)
@@ -133,6 +135,7 @@ class DeviceLoop:
             raise RuntimeError("DeviceLoop: prefill() first")
         if steps < 1 or max(self.ctx) + steps > self.max_len:
             raise ValueError(f"{steps} steps do not fit {self.max_len} tokens")
+        self.model.use_caches(self.caches)
         u = [[uniform(s, self.drawn + t) for s in self.seeds] for t in range(steps)]
         self.u[:steps].copy_(torch.tensor(u, dtype=torch.float32))
         self.step.zero_()

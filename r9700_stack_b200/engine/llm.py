@@ -40,6 +40,7 @@ class LLM:
         num_blocks = ec.num_kv_blocks or (ec.max_batch * blocks_per_seq + 1)
         num_slots = ec.max_batch + 1
         model.alloc_caches(num_blocks, num_slots, ec.kv_block)
+        self.caches = model.held_caches()
         self.scheduler = Scheduler(num_blocks, num_slots, ec.kv_block, ec.max_batch, ec.max_prefill_tokens,
                                    ec.max_model_len)
         max_tokens = max(ec.max_prefill_tokens, ec.max_batch * (1 + ec.spec_tokens))
@@ -61,6 +62,7 @@ class LLM:
 
     def step(self) -> list[Sequence]:
         """One engine step (a prefill chunk or a decode step). Returns sequences that finished."""
+        self.model.use_caches(self.caches)  # the model may serve other engines and loops as well
         k = self.engine_cfg.spec_tokens if self.drafter is not None else 0
         out = self.scheduler.schedule(lookahead=1 + k)
         if out.kind == "idle":

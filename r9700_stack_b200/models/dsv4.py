@@ -75,6 +75,7 @@ class DSV4Workspace(MLAWorkspace):
 
 
 class DSV4LM(MLAMoELM):
+    CACHES = (*MLAMoELM.CACHES, "ng_hist")
     mx_experts = False
 
     def __init__(self, cfg: DSV4Config, par=None, device="cuda", seed: int = 0, comm=None, max_ctx: int = 32768):

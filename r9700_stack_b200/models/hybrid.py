@@ -48,6 +48,20 @@ class NoComm:
 # ------------------------------------------------------------------------------------------------
 # step metadata (device tensors; the runner fills static copies for graph replay)
 # ------------------------------------------------------------------------------------------------
+class PagedCaches:
+    """The caches that a model's forward pass works on, by attribute name. Whoever allocated a set (an engine, a
+    device loop) keeps it and puts it in place before it runs the model, so several of them can share one
+    model's weights, and what their captured graphs point to lives as long as they do."""
+
+    CACHES: tuple[str, ...] = ()
+
+    def held_caches(self) -> dict:
+        return {n: getattr(self, n) for n in self.CACHES}
+
+    def use_caches(self, held: dict) -> None:
+        self.__dict__.update(held)
+
+
 @dataclass
 class StepMeta:
     input_ids: torch.Tensor  # [T] int32
@@ -135,7 +149,9 @@ class Workspace:
         self.acc_len = torch.zeros(max_logit_rows, dtype=torch.int32, device=dev)
 
 
-class HybridLM:
+class HybridLM(PagedCaches):
+    CACHES = ("kv", "ssm", "conv", "qsa_cache")
+
     def __init__(self, cfg: HybridConfig, par: ParallelConfig | None = None, device="cuda", seed: int = 0,
                  comm=None):
         self.cfg = cfg

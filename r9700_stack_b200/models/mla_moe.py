@@ -23,7 +23,7 @@ from .. import _native, knobs
 from ..ops import linear as L
 from ..utils import status as _status
 from .config import ParallelConfig
-from .hybrid import NoComm, StepMeta
+from .hybrid import NoComm, PagedCaches, StepMeta
 from .hybrid_moe import MoEBuffers, moe_ffn
 from .weights import TPFactory, WeightFactory, from_float
 
@@ -132,9 +132,11 @@ class MLAWorkspace:
         self.acc_len = torch.zeros(max_logit_rows, dtype=torch.int32, device=dev)
 
 
-class MLAMoELM:
+class MLAMoELM(PagedCaches):
     """Heads, FFN columns and experts are sharded over ``tp_size`` ranks; the indexer and the latent
     cache are replicated (every rank needs all positions' latent rows for its heads)."""
+
+    CACHES = ("lat", "icache")
 
     mx_experts = True  # routed experts as MXFP4 (subclasses with other expert formats turn this off)
 

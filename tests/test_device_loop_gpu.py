@@ -88,6 +88,46 @@ def test_loop_past_the_length_the_model_was_built_for():
     assert runs[0] == runs[1]
 
 
+def test_loops_and_an_engine_share_a_model():
+    """Taking turns on one model's weights, each gives the tokens that it gives alone."""
+    from r9700_stack_b200.engine.device_loop import DeviceLoop
+    from r9700_stack_b200.engine.llm import LLM
+    from r9700_stack_b200.engine.scheduler import SamplingParams
+    from r9700_stack_b200.models.config import EngineConfig
+    from r9700_stack_b200.models.hybrid import HybridLM
+    from r9700_stack_b200.utils import status
+
+    cfg = _cfg()
+    prompts = [_prompt(n, cfg.vocab, n) for n in (150, 40, 70)]
+    loop = lambda m, i: DeviceLoop(m, 1 + i, 600 - 100 * i, max_prefill_tokens=64)  # noqa: E731
+    engine = lambda m: LLM(cfg, EngineConfig(max_batch=2, max_model_len=300, max_prefill_tokens=64, graph_batch_sizes=[1, 2]), model=m)  # noqa: E731
+    alone = []
+    for i in range(2):
+        lp = loop(HybridLM(cfg, device="cuda", seed=7), i)
+        alone.append([lp.prefill(prompts[: 1 + i])] + lp.decode(60)[0].tolist())
+    alone.append(engine(HybridLM(cfg, device="cuda", seed=7)).generate([prompts[2]], SamplingParams(max_tokens=60))[0])
+    model = HybridLM(cfg, device="cuda", seed=7)
+    loops = [loop(model, 0)]
+    got = [[loops[0].prefill(prompts[:1])] + loops[0].decode(10)[0].tolist()]
+    eng = engine(model)
+    req = eng.add_request(prompts[2], SamplingParams(max_tokens=60))
+    for _ in range(12):
+        eng.step()
+    loops.append(loop(model, 1))
+    got.append([loops[1].prefill(prompts[:2])])
+    for _ in range(5):
+        for lp, out in zip(loops, got):
+            out += lp.decode(10)[0].tolist()
+        for _ in range(10):
+            eng.step()
+    got[1] += loops[1].decode(10)[0].tolist()
+    while eng.has_unfinished():
+        eng.step()
+    torch.cuda.synchronize()
+    status.check()
+    assert got[0] == alone[0] and got[1] == alone[1] and req.output == alone[2]
+
+
 def test_loop_samples_and_repeats():
     from r9700_stack_b200.engine.device_loop import DeviceLoop
     from r9700_stack_b200.engine.scheduler import SamplingParams
