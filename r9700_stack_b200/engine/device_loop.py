@@ -71,9 +71,14 @@ class DeviceLoop:
 
     # ------------------------------------------------------------------------------------------
     def prefill(self, prompts: list[list[int]], params: list[SamplingParams] | None = None) -> list[int]:
-        """Run the prompts (one a sequence, in chunks) and draw each sequence's first token."""
+        """Run the prompts (one a sequence, in chunks) and draw each sequence's first token.
+
+        Of ``params``, temperature, top_k, top_p, min_p and seed count. How long a sequence gets is the caller's
+        affair: :meth:`decode` draws as many tokens as it is told to for all of them, past an end token too."""
         if len(prompts) != self.seqs or any(not 1 <= len(p) < self.max_len for p in prompts):
             raise ValueError(f"need {self.seqs} prompts of 1 to {self.max_len - 1} tokens")
+        if any(not 0 <= min(p) <= max(p) < self.model.cfg.vocab for p in prompts):
+            raise ValueError("a prompt's token is outside the vocabulary")
         if self.ctx:
             raise RuntimeError("DeviceLoop: prefill() starts a new loop's sequences once")
         params = params or [SamplingParams()] * self.seqs
