@@ -34,6 +34,7 @@ NVCC_FLAGS = ARCH_FLAGS + [
     "-fno-strict-aliasing",
 ]
 CXX_FLAGS = ["-O3", "-std=c++17", "-DNDEBUG"]
+CXX_RUNTIME = "-l:libstdc++.so.6"
 
 _lock = threading.Lock()
 _loaded = False
@@ -51,7 +52,7 @@ def _source_hash() -> str:
             h.update(os.path.basename(p).encode())
             with open(p, "rb") as f:
                 h.update(f.read())
-    h.update(" ".join(NVCC_FLAGS).encode())
+    h.update(" ".join([*NVCC_FLAGS, *CXX_FLAGS, CXX_RUNTIME]).encode())
     return h.hexdigest()
 
 
@@ -77,7 +78,7 @@ def _cxx_runtime() -> list[str]:
         found = subprocess.run(["g++", "-print-file-name=libstdc++.so.6"], capture_output=True, text=True).stdout.strip()
     except OSError:
         return []
-    return ["-l:libstdc++.so.6"] if os.path.isabs(found) else []
+    return [CXX_RUNTIME] if os.path.isabs(found) else []
 
 
 def build(verbose: bool = False) -> str:
