@@ -52,10 +52,6 @@ class HybridConfig:
     # indexer of qsa_heads x 128 query heads against mean-pooled group keys (0 = dense attention)
     qsa_topk: int = 0
     qsa_heads: int = 4
-    # sliding window of the full-attention layers, in tokens, and the first tokens of a sequence that stay
-    # visible (0 = the whole context)
-    attn_window: int = 0
-    attn_sinks: int = 0
     # hyper-connections: HC residual streams, sigmoid-gated mix into every block (0 = plain residual)
     hc_streams: int = 0
     init_std: float = 0.02
@@ -64,6 +60,10 @@ class HybridConfig:
     mtp_layers: int = 0
     drafter: str = ""  # "" | "block" | "mtp"
     draft_block: int = 8
+    # sliding window of the full-attention layers, in tokens, and the first tokens of a sequence that stay
+    # visible (0 = the whole context)
+    attn_window: int = 0
+    attn_sinks: int = 0
 
     def is_attention(self, i: int) -> bool:
         return (i + 1) % self.full_attn_interval == 0
