@@ -175,6 +175,81 @@ def test_loop_refusals():
         HybridLM(_cfg(qsa_topk=4), device="cuda")
 
 
+def _agree(a, b):
+    """Length of the common prefix: other shapes add in other orders, so a rare near-tie may flip."""
+    return next((i for i, (x, y) in enumerate(zip(a, b)) if x != y), min(len(a), len(b)))
+
+
+@pytest.mark.parametrize("kind", ["moe", "heads of 128", "no window"])
+def test_loop_on_other_models(kind):
+    """One greedy request at a time, far past the window: the engine's kernels on the engine's shapes, so its tokens."""
+    from r9700_stack_b200.engine.device_loop import DeviceLoop
+    from r9700_stack_b200.engine.llm import LLM, build_model
+    from r9700_stack_b200.engine.scheduler import SamplingParams
+    from r9700_stack_b200.models.config import EngineConfig, ParallelConfig, tiny_moe
+    from r9700_stack_b200.utils import status
+
+    cfg = {"moe": tiny_moe(attn_window=50, attn_sinks=4), "heads of 128": _cfg(head_dim=128, attn_window=70),
+           "no window": _cfg(attn_window=0, attn_sinks=0)}[kind]
+    model = build_model(cfg, ParallelConfig(), torch.device("cuda"), seed=7)
+    for prompt in (_prompt(90, cfg.vocab), _prompt(33, cfg.vocab, 6)):
+        llm = LLM(cfg, EngineConfig(max_batch=1, max_model_len=512, max_prefill_tokens=64, graph_batch_sizes=[1]), model=model)
+        want = llm.generate([prompt], SamplingParams(max_tokens=100))[0]
+        loop = DeviceLoop(model, 1, 512, max_prefill_tokens=64)
+        got = loop.prefill([prompt]) + loop.decode(99)[0][:, 0].tolist()
+        torch.cuda.synchronize()
+        status.check()
+        assert got == want
+
+
+@pytest.mark.parametrize("method", ["ngram", "mtp", "block", "dspark"])
+def test_windowed_model_with_speculation(method):
+    """Verification of drafts under a window that most of the sequence has left, captured graphs and ragged steps."""
+    from r9700_stack_b200.engine.llm import LLM
+    from r9700_stack_b200.engine.scheduler import SamplingParams
+    from r9700_stack_b200.models.config import EngineConfig
+    from r9700_stack_b200.utils import status
+
+    cfg = _cfg(gdn_state_dtype="fp32", attn_window=40)
+    prompts = [_prompt(n, cfg.vocab, n) for n in (37, 80, 12)]
+    run = lambda **kw: LLM(cfg, EngineConfig(max_batch=3, max_model_len=256, max_prefill_tokens=64,  # noqa: E731
+                                             graph_batch_sizes=[1, 2, 4], **kw), seed=7)
+    want = run().generate(prompts, SamplingParams(max_tokens=20))
+    llm = run(spec_tokens=3, spec_method=method)
+    got = llm.generate(prompts, SamplingParams(max_tokens=20))
+    torch.cuda.synchronize()
+    status.check()
+    for a, b in zip(got, want):
+        assert len(a) == 20 and _agree(a, b) >= 16, (a, b)
+    assert llm.spec_stats["steps"] > 0
+
+
+def test_windowed_model_on_scripted_drafts():
+    """Right and wrong drafts: rejected tokens leave no trace in what the window sees later."""
+    from r9700_stack_b200.engine.llm import LLM
+    from r9700_stack_b200.engine.scheduler import SamplingParams
+    from r9700_stack_b200.models.config import EngineConfig
+    from r9700_stack_b200.spec.drafters import ScriptedDrafter
+    from r9700_stack_b200.utils import status
+
+    cfg = _cfg(gdn_state_dtype="fp32", attn_window=40)
+    prompts = [_prompt(n, cfg.vocab, n) for n in (37, 80, 12)]
+    ec = dict(max_batch=3, max_model_len=256, max_prefill_tokens=64, graph_batch_sizes=[1, 2, 4])
+    want = LLM(cfg, EngineConfig(**ec), seed=7).generate(prompts, SamplingParams(max_tokens=60))
+    drafter = ScriptedDrafter(4, {}, pad=0, corrupt_every=3)
+    llm = LLM(cfg, EngineConfig(spec_tokens=4, **ec), seed=7, drafter=drafter)
+    seqs = [llm.add_request(p, SamplingParams(max_tokens=60)) for p in prompts]
+    for s, ref in zip(seqs, want):
+        drafter.script[s.seq_id] = ref
+    while llm.has_unfinished():
+        llm.step()
+    torch.cuda.synchronize()
+    status.check()
+    for s, ref in zip(seqs, want):
+        assert _agree(s.output, ref) >= 16, (s.output, ref)
+    assert 0 < llm.spec_stats["accepted"] < llm.spec_stats["drafted"]
+
+
 def test_engine_device_sampling():
     from r9700_stack_b200.engine.llm import LLM
     from r9700_stack_b200.engine.scheduler import SamplingParams
