@@ -760,7 +760,7 @@ void sample_logits(torch::Tensor logits, torch::Tensor u, torch::Tensor temperat
   auto slice_of = [&](int c) { return ((V + c - 1) / c + 3) / 4 * 4; };
   auto wave = [&](int c) { return c == 16 ? sms * 3 / 2 : sms * 7 / 4; };
   int least = 1;
-  while (slice_of(least) > 65532) least *= 2;
+  while (slice_of(least) > MAX_SLICE) least *= 2;
   int C = sm::MAX_CLUSTER;
   while (C > least && (slice_of(C) < 4096 || R * C > wave(C))) C /= 2;
   // Slices held in shared memory are read once; as long as two of them fit an SM and one wave takes all rows
