@@ -744,11 +744,14 @@ __global__ void __launch_bounds__(wd::THREADS, 2)
 //
 // What bounds it: 8192 tokens, 24 / 4 heads of 256, window 4096: 890 to 975 us with the card's clocks, 850 to
 // 930 TFLOP/s of useful products, 0.51 to 0.55 of the bf16 rate (the tensor pipe is busy 0.46 of the time at the
-// 8-bit rate, on two planes). A key tile takes about 2900 cycles: 2050 of MMA at the least, beside a softmax of
-// about 2200 (1024 of them the exponential unit's 16 a cycle) whose scores, maxima and probabilities follow one
-// another.
-// Ragged prompts, 3850 tokens, 32 / 8 heads of 128, window 1024: 147 us; ten key tiles a CTA do not hide
-// its start (page and length reads, queries) and end, 13000 cycles together.
+// 8-bit rate, on two planes). Stamps of all 1568 CTAs at 1.8 GHz: 141000 cycles a CTA. Its start (page
+// and length reads, queries) takes 14700, 33 key tiles 100000 and its end (last product, gate, output) 25700;
+// nothing covers a start or an end, as one CTA fills an SM. A tile takes 3020 on average: 2510 where O stays as
+// it is, 3000 where some row's is rescaled (three in four), 3500 at the masked edges (two a CTA). 2050 of them are
+// MMA at the least, beside a softmax chain of about 2200 (1024 the exponential unit's 16 a cycle), 2600 with its
+// wait for the scores.
+// Ragged prompts, 3850 tokens, 32 / 8 heads of 128, window 1024: 148 us. A CTA of nine tiles takes 40000 cycles:
+// 27700 in the tiles, 3080 each, 7500 before them and 2800 after.
 // Shares of 1 / 2 / 4 / 8 CTAs for 16 sequences x 1..8 drafts, 16 / 2 heads: 34 / 27 / 21 / 44 us.
 // ------------------------------------------------------------------------------------------------
 namespace wc {
